@@ -263,6 +263,78 @@ size_t qm_prelayout_b_bytes(int n, int k);
 int qm_prelayout_b(const void *B, void *B_pre, int n, int k, void *stream);
 int qm_gemm_s4_prelaid(const void *A, const void *B_pre, void *C, int m, int n, int k, void *stream);
 
+/*
+ * ---- 4-bit weights with group scales, 16-bit activations ------------------------------------------------------------
+ *
+ *   out[r][c] = sum over g of scale[c][g] * ( sum over i in group g of X[r][i] * q[c][i] )
+ *
+ * q are the packed s4 codes of B (the layout of every other entry point: n x k/2 bytes, low nibble first), group g holds the
+ * elements g * group .. g * group + group - 1 of a row (the last group of a row may be short), and scale is a row-major
+ * n x ceil(k / group) matrix.  The reference has no counterpart: its only product is s4 x s4.
+ */
+typedef enum qm_type {
+    QM_TYPE_F32 = 0,
+    QM_TYPE_F16 = 1,
+    QM_TYPE_BF16 = 2
+} qm_type_t;
+
+/*
+ * X (m x k, row pitch ldx elements) times the transpose of B into out (m x n, row pitch ldo elements); X and out are both
+ * QM_TYPE_F16 or both QM_TYPE_BF16 (`type`), the scales have that type or QM_TYPE_F32, group is 32, 64, 128 or 256, k is even.
+ * Sums are fp32 and are rounded to `type` once.  out is fully overwritten; k == 0 zeroes it.
+ */
+int qm_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group, void *out,
+               int64_t ldo, int m, int n, int k, void *stream);
+
+/*
+ * The same product with one weight matrix per expert, over rows that are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1
+ * of X are multiplied with matrix e of B (experts x n x k/2 bytes) and scales (experts x n x ceil(k / group)).  offsets
+ * (experts + 1 ints, device memory, not decreasing) is read by the kernel: a launch does not depend on its values, so it can be
+ * captured.  Offsets outside [0, rows] are clamped; rows of out that belong to no expert are left as they were.
+ */
+int qm_moe_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group,
+                   const int *offsets, int experts, void *out, int64_t ldo, int rows, int n, int k, void *stream);
+
+/*
+ * W (rows x k, row pitch ldw elements, any qm_type_t) -> packed codes (rows x k/2 bytes) and scales (rows x ceil(k / group),
+ * of W's type or QM_TYPE_F32): per group, scale = the largest |w| times the fp32 value of 1/7, rounded to the scales' type, and
+ * code = w / scale rounded to the nearest integer (the exact quotient, ties to even), clamped to [-8, 7].  A group of zeros
+ * has scale 0 and codes 0; a group with an infinity or a NaN has a scale that is not finite (NaN where there is a NaN) and codes 0.
+ * group and k as in qm_gemm_w4.
+ */
+int qm_quantize_w4(const void *W, int type, int64_t ldw, void *packed, void *scales, int scale_type, int64_t rows, int64_t k, int group,
+                   void *stream);
+
+/*
+ * ---- tokens to experts and back ---------------------------------------------------------------------------------------
+ *
+ * `ids` (tokens x top_k, int32 or int64 by id_bytes = 4 or 8) names the expert of every assignment; one outside [0, experts)
+ * is dropped.  qm_moe_sort writes
+ *   offsets[e]   how many assignments go to experts below e (experts + 1 ints; offsets[experts] = all that are not dropped),
+ *   slots[t][j]  the assignment's row in expert order, -1 where it is dropped; within an expert the order is that of
+ *                (t, j), so equal inputs give equal results,
+ *   xs[slots[t][j]] = X[t]   (`hidden` elements of any qm_type_t; xs holds tokens x top_k rows with pitch ldxs; rows from
+ *                offsets[experts] on are left as they were).
+ */
+int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_bytes, int experts, void *xs, int64_t ldxs, int *offsets,
+                int *slots, int tokens, int top_k, int hidden, void *stream);
+
+/*
+ * y[t] = sum over j of weights[t][j] * ys[slots[t][j]], in fp32 in the order of j, rounded once.  Slots outside [0, rows)
+ * add nothing (a token without any gets zeros).  weights (tokens x top_k, of ys's type or QM_TYPE_F32) may be NULL: all ones,
+ * which is the gradient of qm_moe_sort with respect to X (ys = the gradient of xs).
+ */
+int qm_moe_combine(const void *ys, int type, int64_t ldys, int rows, const int *slots, const void *weights, int weight_type, void *y,
+                   int64_t ldy, int tokens, int top_k, int hidden, void *stream);
+
+/*
+ * The gradients of qm_moe_combine: dys[slots[t][j]] = weights[t][j] * dy[t] (rows that no slot names are left as they were) and
+ * dweights[t][j] = <dy[t], ys[slots[t][j]]> in fp32, rounded to weight_type (0 for a slot outside [0, rows)).
+ */
+int qm_moe_combine_grad(const void *dy, int64_t lddy, const void *ys, int64_t ldys, int type, int rows, const int *slots,
+                        const void *weights, int weight_type, void *dys, int64_t lddys, void *dweights, int tokens, int top_k,
+                        int hidden, void *stream);
+
 /* What the dispatcher would run for (m, n, k): fills *opts with the resolved choices. */
 int qm_plan(int m, int n, int k, qm_gemm_opts_t *opts);
 

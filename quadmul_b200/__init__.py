@@ -8,6 +8,9 @@ Host-side mirror of the reference's Python surface:
   pack(x)                  the reference test's `pack_b` (test.py:6-15) as a CUDA kernel.
   unpack(p)                the reference's host `unpack_int4_matrix` (kernel.cu:389-408) as a CUDA kernel.
 
+Beyond the reference, for 16-bit activations and mixtures of experts (w4.py, moe.py): gemm_w4, moe_gemm_w4, quantize_w4,
+moe_sort, moe_combine, their gradients and moe_linear_w4.
+
 Everything runs through the C ABI in include/quadmul_b200.h (libquadmul_b200.so, built in-tree
 with nvcc).  torch is used for device memory and streams only.  There is no CPU or library
 fallback: without the shared object the import fails, and every error status raises.
@@ -33,6 +36,14 @@ __all__ = [
     "unshard_c",
     "QuadmulError",
     "launch_count",
+    "gemm_w4",
+    "moe_gemm_w4",
+    "quantize_w4",
+    "moe_sort",
+    "moe_sort_grad",
+    "moe_combine",
+    "moe_combine_grad",
+    "moe_linear_w4",
 ]
 
 _launches = 0  # kernels this package launched (one per call below; split-K adds none)
@@ -47,6 +58,11 @@ except Exception:  # not built, or built against another torch
 
 def launch_count() -> int:
     return _launches
+
+
+def _count(launches: int) -> None:
+    global _launches
+    _launches += launches
 
 
 def _torch():
@@ -313,3 +329,7 @@ def unshard_c(slabs, c, m: int, n: int, world: int, slab_stride: int) -> None:
         st = LIB.qm_unshard_c(slabs.data_ptr(), c.data_ptr(), m, n, world, slab_stride, _stream_of(c))
     check(st, "unshard_c")
     _launches += 1
+
+
+from .w4 import gemm_w4, moe_gemm_w4, quantize_w4  # noqa: E402
+from .moe import moe_combine, moe_combine_grad, moe_linear_w4, moe_sort, moe_sort_grad  # noqa: E402

@@ -60,6 +60,12 @@ SIGNATURES = {
     "qm_prelayout_b_bytes": (ctypes.c_size_t, [_i, _i]),
     "qm_prelayout_b": (_i, [_vp, _vp, _i, _i, _vp]),
     "qm_gemm_s4_prelaid": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "qm_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i64, _i, _i, _i, _vp]),
+    "qm_moe_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
+    "qm_quantize_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i64, _i64, _i, _vp]),
+    "qm_moe_sort": (_i, [_vp, _i, _i64, _vp, _i, _i, _vp, _i64, _vp, _vp, _i, _i, _i, _vp]),
+    "qm_moe_combine": (_i, [_vp, _i, _i64, _i, _vp, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
+    "qm_moe_combine_grad": (_i, [_vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _i, _vp, _i64, _vp, _i, _i, _i, _vp]),
     "qm_flag_signal": (_i, [_vp, _i, _vp]),
     "qm_flags_wait": (_i, [_vp, _i, _i, _i, _vp]),
 }
@@ -68,6 +74,7 @@ SIGNATURES = {
 WRAPPER_MANGLED = "_Z7wrapperPvS_S_iiiP11CUstream_st"
 
 QM_OK = 0
+QM_TYPE_F32, QM_TYPE_F16, QM_TYPE_BF16 = 0, 1, 2
 QM_KERNEL_AUTO, QM_KERNEL_TC, QM_KERNEL_SIMT, QM_KERNEL_GEMV, QM_KERNEL_RMMA = 0, 1, 2, 3, 4
 
 

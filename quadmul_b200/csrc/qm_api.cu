@@ -240,6 +240,8 @@ int gemm_dispatch(const void *A, const void *B, void *C, int m, int n, int k, in
 
 }  // namespace
 
+int device_ctx(DeviceCtx **out) { return ensure_ctx(out); }
+
 int record_cuda_error(cudaError_t e, const char *what)
 {
     t_last_error = std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")";

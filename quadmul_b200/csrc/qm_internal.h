@@ -131,10 +131,62 @@ int unshard_launch(const int32_t *slabs, int32_t *C, int m, int n, int world, in
 int flag_signal_launch(int *flag, int value, cudaStream_t s);
 int flags_wait_launch(const int *flags, int count, int value, int timeout_ms, int *status, cudaStream_t s);
 
+// ---- 4-bit weights with group scales (qm_api_w4.cu checks the arguments) ----------------------------------------------
+struct W4Args {
+    const void *X;  // rows x ldx, `type`
+    int type;       // QM_TYPE_F16 or QM_TYPE_BF16, also of out
+    int64_t ldx;
+    const uint8_t *B;    // experts x n x k/2
+    const void *scales;  // experts x n x groups, scale_type
+    int scale_type, group;
+    const int *offsets;  // experts + 1, device memory; NULL: one matrix for all rows
+    int experts;         // 1 without offsets
+    void *out;
+    int64_t ldo;
+    int rows, n, k;
+    cudaStream_t stream;
+};
+int w4_simt_launch(const W4Args &a);  // qm_w4_simt.cu
+int quantize_w4_launch(const void *W, int type, int64_t ldw, uint8_t *packed, void *scales, int scale_type, int64_t rows, int64_t k, int group,
+                       cudaStream_t s);  // qm_w4_quant.cu
+
+// ---- qm_moe.cu: tokens to experts and back ------------------------------------------------------------------------------
+struct MoeSortArgs {
+    const void *X;
+    int type;
+    int64_t ldx;
+    const void *ids;
+    int id_bytes, experts;
+    void *xs;
+    int64_t ldxs;
+    int *offsets, *slots;
+    int tokens, top_k, hidden;
+    cudaStream_t stream;
+};
+int moe_sort_launch(const MoeSortArgs &a);
+struct MoeCombineArgs {
+    const void *dy;  // gradient only
+    int64_t lddy;
+    const void *ys;
+    int64_t ldys;
+    int type, rows;
+    const int *slots;
+    const void *weights;  // NULL: all ones (not in the gradient)
+    int weight_type;
+    void *out;  // y, or dys
+    int64_t ldo;
+    void *dweights;  // gradient only
+    int tokens, top_k, hidden;
+    cudaStream_t stream;
+};
+int moe_combine_launch(const MoeCombineArgs &a);
+int moe_combine_grad_launch(const MoeCombineArgs &a);
+
 // qm_api.cu
 // Column split of n over `world` ranks: whole units of 128 columns where n allows, the last ranks
 // take the remainder units.
 void nshard_range(int n, int world, int rank, int *begin, int *count);
+int device_ctx(DeviceCtx **out);  // the current device's state, created on first use
 int record_cuda_error(cudaError_t e, const char *what);  // returns QM_ERR_CUDA, stores the text
 
 }  // namespace qm
