@@ -14,7 +14,7 @@ bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(
 
 int check_w4(const W4Args &a)
 {
-    if (a.rows < 0 || a.n < 0 || a.k < 0 || (a.k & 1) || a.experts < 0) return QM_ERR_SHAPE;
+    if (a.rows < 0 || a.n < 0 || a.k < 0 || (a.k & 1) || a.experts < 0 || a.experts > kMaxExperts) return QM_ERR_SHAPE;
     if (a.type != QM_TYPE_F16 && a.type != QM_TYPE_BF16) return QM_ERR_ARG;
     if (a.scale_type != QM_TYPE_F32 && a.scale_type != a.type) return QM_ERR_ARG;
     if (!known_group(a.group)) return QM_ERR_ARG;
@@ -29,6 +29,12 @@ int w4_dispatch(const W4Args &a)
 {
     int st = check_w4(a);
     if (st != QM_OK || a.rows == 0 || a.n == 0 || a.experts == 0) return st;
+    DeviceCtx *ctx = nullptr;
+    st = device_ctx(&ctx);
+    if (st != QM_OK) return st;
+    const int average = a.rows / (a.experts < a.rows ? a.experts : a.rows);
+    if (average <= (a.offsets ? 8 : 16) && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
+    if (w4_tc_eligible(a)) return w4_tc_launch(a, *ctx);
     return w4_simt_launch(a);
 }
 
@@ -75,7 +81,7 @@ int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_by
     int st = check_moe(type, tokens, top_k, hidden);
     if (st != QM_OK) return st;
     if (id_bytes != 4 && id_bytes != 8) return QM_ERR_ARG;
-    if (experts < 0 || experts > 4096) return QM_ERR_SHAPE;
+    if (experts < 0 || experts > kMaxExperts) return QM_ERR_SHAPE;
     if (!offsets) return QM_ERR_NULL;
     const bool some = tokens > 0 && top_k > 0;
     if (some && (!ids || !slots || (hidden > 0 && (!X || !xs)))) return QM_ERR_NULL;

@@ -54,5 +54,120 @@ inline int launched(const char *what)
     return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
 }
 
+// The experts' segments, from offsets that may be anything: seg[e] (e = 0 .. experts) is the running maximum of the offsets
+// clamped to [0, rows], so expert e has the rows [seg[e], seg[e + 1]); tiles[e] is how many tiles of `tile` rows the experts
+// below e have.  Run by one warp; seg and tiles are shared memory, to be read after a barrier.
+__device__ __forceinline__ void scan_segments(const int *__restrict__ offsets, int experts, int rows, int tile, int *seg, int *tiles, int lane)
+{
+    int top = 0, sum = 0;  // running maximum and sum of what came before
+    for (int base = 0; base <= experts; base += 32) {
+        const int e = base + lane;
+        int v = e <= experts ? max(0, min(__ldg(offsets + e), rows)) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            if (lane >= d) v = max(v, o);
+        }
+        v = max(v, top);
+        int before = __shfl_up_sync(0xFFFFFFFFu, v, 1);  // seg[e - 1]
+        if (lane == 0) before = base == 0 ? v : top;
+        int t = (v - before + tile - 1) / tile;  // tiles of expert e - 1 (none before expert 0)
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xFFFFFFFFu, t, d);
+            if (lane >= d) t += o;
+        }
+        t += sum;
+        if (e <= experts) seg[e] = v, tiles[e] = t;
+        top = __shfl_sync(0xFFFFFFFFu, v, 31);
+        sum = __shfl_sync(0xFFFFFFFFu, t, 31);
+    }
+}
+
+// The expert that has tile p: the last e with tiles[e] <= p (p < tiles[experts]).
+__device__ __forceinline__ int expert_of_tile(const int *tiles, int experts, int p)
+{
+    int lo = 0, hi = experts;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles[mid] <= p) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// (a & mask) ^ flip in one instruction
+__device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t mask, uint32_t flip)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(a), "r"(mask), "r"(flip));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, Tag<__nv_bfloat16>)
+{
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, Tag<__half>)
+{
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+
+// Eight codes e0 .. e7 of one word -> four pairs (e0, e4), (e1, e5), (e2, e6), (e3, e7) of 16-bit floats, exactly.  A nibble n is
+// the code q = (n ^ 8) - 8.  n ^ 8 put into the last mantissa bits of a power of two whose last place is 1 (bf16 128, fp16 1024)
+// reads as that power plus q + 8, so one subtraction leaves q; fp16 has room to take a nibble four bits up (its last place then
+// counts 1/16) and saves shifts.
+__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = fma2(and_xor(w >> (4 * i), 0x000F000Fu, 0x43084308u), 0x3F803F80u, 0xC308C308u, tag);  // x 1 - 136
+}
+__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__half> tag)
+{
+    const uint32_t w8 = w >> 8;
+    c[0] = fma2(and_xor(w, 0x000F000Fu, 0x64086408u), 0x3C003C00u, 0xE408E408u, tag);   // x 1 - 1032
+    c[1] = fma2(and_xor(w, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u, tag);   // x 1/16 - 72
+    c[2] = fma2(and_xor(w8, 0x000F000Fu, 0x64086408u), 0x3C003C00u, 0xE408E408u, tag);
+    c[3] = fma2(and_xor(w8, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u, tag);
+}
+
+// The same eight codes in their own order: (e0, e1), (e2, e3), (e4, e5), (e6, e7).  A byte permute puts a byte's two nibbles into
+// the two halves: bf16 takes the high one from a copy of the word shifted by four, fp16 takes it where it is (see above).
+__device__ __forceinline__ void codes_in_order(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
+{
+    const uint32_t w4 = w >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        c[j] = fma2(and_xor(__byte_perm(w, w4, 0x4400 + 0x1111 * j), 0x000F000Fu, 0x43084308u), 0x3F803F80u, 0xC308C308u, tag);
+}
+__device__ __forceinline__ void codes_in_order(uint32_t w, uint32_t (&c)[4], Tag<__half> tag)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        c[j] = fma2(and_xor(__byte_perm(w, 0u, 0x1111 * j), 0x00F0000Fu, 0x64806408u), 0x2C003C00u, 0xD480E408u, tag);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, Tag<__nv_bfloat16>)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, Tag<__half>)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v, Tag<__nv_bfloat16>) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 unpack2(uint32_t v, Tag<__half>)
+{
+    return make_float2(__half2float(__ushort_as_half((unsigned short)v)), __half2float(__ushort_as_half((unsigned short)(v >> 16))));
+}
+
 }  // namespace w4
 }  // namespace qm
