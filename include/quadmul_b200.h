@@ -290,7 +290,7 @@ int qm_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *
  * The same product with one weight matrix per expert, over rows that are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1
  * of X are multiplied with matrix e of B (experts x n x k/2 bytes) and scales (experts x n x ceil(k / group)).  offsets
  * (experts + 1 ints, device memory, not decreasing) is read by the kernel: a launch does not depend on its values, so it can be
- * captured.  Offsets outside [0, rows] are clamped; rows of out that belong to no expert are left as they were.
+ * captured.  experts is at most 4096.  Offsets outside [0, rows] are clamped; rows of out that belong to no expert are left as they were.
  */
 int qm_moe_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group,
                    const int *offsets, int experts, void *out, int64_t ldo, int rows, int n, int k, void *stream);
@@ -315,9 +315,12 @@ int qm_quantize_w4(const void *W, int type, int64_t ldw, void *packed, void *sca
  *                (t, j), so equal inputs give equal results,
  *   xs[slots[t][j]] = X[t]   (`hidden` elements of any qm_type_t; xs holds tokens x top_k rows with pitch ldxs; rows from
  *                offsets[experts] on are left as they were).
+ * Many assignments need a workspace (device memory, 4-byte aligned; qm_moe_sort_workspace_bytes says how much, 0 = none,
+ * QM_ERR_WORKSPACE if it is smaller).  experts and top_k are at most 4096.
  */
 int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_bytes, int experts, void *xs, int64_t ldxs, int *offsets,
-                int *slots, int tokens, int top_k, int hidden, void *stream);
+                int *slots, int tokens, int top_k, int hidden, void *workspace, size_t workspace_bytes, void *stream);
+size_t qm_moe_sort_workspace_bytes(int tokens, int top_k, int experts);
 
 /*
  * y[t] = sum over j of weights[t][j] * ys[slots[t][j]], in fp32 in the order of j, rounded once.  Slots outside [0, rows)

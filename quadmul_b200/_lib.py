@@ -63,7 +63,8 @@ SIGNATURES = {
     "qm_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i64, _i, _i, _i, _vp]),
     "qm_moe_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
     "qm_quantize_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i64, _i64, _i, _vp]),
-    "qm_moe_sort": (_i, [_vp, _i, _i64, _vp, _i, _i, _vp, _i64, _vp, _vp, _i, _i, _i, _vp]),
+    "qm_moe_sort": (_i, [_vp, _i, _i64, _vp, _i, _i, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
+    "qm_moe_sort_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
     "qm_moe_combine": (_i, [_vp, _i, _i64, _i, _vp, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
     "qm_moe_combine_grad": (_i, [_vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _i, _vp, _i64, _vp, _i, _i, _i, _vp]),
     "qm_flag_signal": (_i, [_vp, _i, _vp]),

@@ -40,7 +40,7 @@ int w4_dispatch(const W4Args &a)
 
 int check_moe(int type, int tokens, int top_k, int hidden)
 {
-    if (tokens < 0 || top_k < 0 || hidden < 0 || (int64_t)tokens * top_k > INT_MAX) return QM_ERR_SHAPE;
+    if (tokens < 0 || top_k < 0 || top_k > kMaxExperts || hidden < 0 || (int64_t)tokens * top_k > INT_MAX) return QM_ERR_SHAPE;
     return w4::known_type(type) ? QM_OK : QM_ERR_ARG;
 }
 
@@ -76,7 +76,7 @@ int qm_quantize_w4(const void *W, int type, int64_t ldw, void *packed, void *sca
 }
 
 int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_bytes, int experts, void *xs, int64_t ldxs, int *offsets, int *slots,
-                int tokens, int top_k, int hidden, void *stream)
+                int tokens, int top_k, int hidden, void *workspace, size_t workspace_bytes, void *stream)
 {
     int st = check_moe(type, tokens, top_k, hidden);
     if (st != QM_OK) return st;
@@ -89,7 +89,17 @@ int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_by
     if (!aligned_to(offsets, 4) || !aligned_to(slots, 4) || !aligned_to(ids, id_bytes) || !aligned_to(X, w4::type_bytes(type)) ||
         !aligned_to(xs, w4::type_bytes(type)))
         return QM_ERR_ALIGN;
-    return moe_sort_launch({X, type, ldx, ids, id_bytes, experts, xs, ldxs, offsets, slots, tokens, top_k, hidden, static_cast<cudaStream_t>(stream)});
+    const size_t need = moe_sort_workspace(tokens, top_k, experts);
+    if (need && (!workspace || workspace_bytes < need)) return QM_ERR_WORKSPACE;
+    if (need && !aligned_to(workspace, 4)) return QM_ERR_ALIGN;
+    return moe_sort_launch({X, type, ldx, ids, id_bytes, experts, xs, ldxs, offsets, slots, tokens, top_k, hidden, static_cast<int *>(workspace),
+                            static_cast<cudaStream_t>(stream)});
+}
+
+size_t qm_moe_sort_workspace_bytes(int tokens, int top_k, int experts)
+{
+    if (tokens < 0 || top_k < 0 || experts < 0) return 0;
+    return moe_sort_workspace(tokens, top_k, experts);
 }
 
 int qm_moe_combine(const void *ys, int type, int64_t ldys, int rows, const int *slots, const void *weights, int weight_type, void *y, int64_t ldy,

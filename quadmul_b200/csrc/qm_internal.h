@@ -168,8 +168,10 @@ struct MoeSortArgs {
     int64_t ldxs;
     int *offsets, *slots;
     int tokens, top_k, hidden;
+    int *workspace;  // moe_sort_workspace() bytes
     cudaStream_t stream;
 };
+size_t moe_sort_workspace(int tokens, int top_k, int experts);
 int moe_sort_launch(const MoeSortArgs &a);
 struct MoeCombineArgs {
     const void *dy;  // gradient only

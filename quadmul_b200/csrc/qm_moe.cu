@@ -1,122 +1,339 @@
 // Tokens to experts and back: a stable counting sort of the assignments with the copy of their rows, the weighted sum that
-// brings the experts' rows back, and the gradients of both.  All of it is bound by memory.
+// brings the experts' rows back, and the gradients of both.  All of it is bound by memory: rows move in 16-byte pieces with
+// several in flight per thread, and nothing is read twice but indices.
+//
+// Sorting.  slot(t, j) = (assignments to lower experts) + (earlier assignments to the same expert): a counting sort, stable, without
+// atomics on anything that decides an order.  Up to kFewIds assignments take ONE launch: every block counts all ids itself
+// (they are L2 hits), which costs a microsecond or two and saves two launches and a workspace.  More take three: counts per
+// block of assignments, a scan of the counts over the blocks, and the placing.
+#include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
 namespace qm {
 
 using namespace w4;
 
-// Offsets and slots.  One warp walks the assignments in order; lanes with the same expert are ranked by a match, so the
-// order within an expert is the order of the assignments.
-template <typename I>
-__global__ void __launch_bounds__(1024) moe_slots_kernel(const I *__restrict__ ids, int experts, int count, int *__restrict__ offsets,
-                                                         int *__restrict__ slots)
-{
-    extern __shared__ int next[];  // experts + 1
-    for (int e = threadIdx.x; e <= experts; e += blockDim.x) next[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += blockDim.x) {
-        const I id = ids[i];
-        if (id >= 0 && id < (I)experts) atomicAdd(&next[(int)id + 1], 1);
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kFewIds = 16384;
+constexpr int kBlocks = 148 * 4;  // blocks that share the assignments
+
+// VEC elements of T that move together: 16 bytes, or one element where rows are not on 16-byte boundaries.
+template <typename T, int VEC>
+struct Piece {
+    static_assert(VEC == 1 || VEC * sizeof(T) == 16, "piece");
+    T v[VEC];
+    __device__ __forceinline__ void load(const T *p)
+    {
+        if constexpr (VEC == 1) v[0] = __ldcs(p);
+        else *reinterpret_cast<uint4 *>(v) = __ldcs(reinterpret_cast<const uint4 *>(p));
     }
-    __syncthreads();
-    if (threadIdx.x == 0)
-        for (int e = 0; e < experts; ++e) next[e + 1] += next[e];
-    __syncthreads();
-    for (int e = threadIdx.x; e <= experts; e += blockDim.x) offsets[e] = next[e];
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    const int lane = threadIdx.x;
-    for (int base = 0; base < count; base += 32) {
-        const int i = base + lane;
-        const I id = i < count ? ids[i] : (I)-1;
-        const bool live = id >= 0 && id < (I)experts;
-        const int e = live ? (int)id : -1;
-        const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
-        const int rank = __popc(same & ((1u << lane) - 1u));
-        const int at = live ? next[e] + rank : -1;
-        __syncwarp();
-        if (live && rank == 0) next[e] += __popc(same);
-        __syncwarp();
-        if (i < count) slots[i] = at;
+    __device__ __forceinline__ void store(T *p) const
+    {
+        if constexpr (VEC == 1) __stcs(p, v[0]);
+        else __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(v));
+    }
+};
+
+__device__ __forceinline__ int expert_id(int64_t id, int experts) { return id >= 0 && id < experts ? (int)id : -1; }
+
+// Adds each lane's expert (-1: none) to counts[]: one atomic per expert of the warp.
+__device__ __forceinline__ void count_ids(int *counts, int e, int lane)
+{
+    const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+    if (e >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + e, __popc(same));
+}
+
+// Ids [first, last) -> how many go to each expert, in counts[0 .. experts); the whole block.
+template <typename I>
+__device__ __forceinline__ void count_range(const I *__restrict__ ids, int64_t first, int64_t last, int experts, int *counts)
+{
+    const int lane = threadIdx.x & 31;
+    for (int64_t base = first + (threadIdx.x & ~31); base < last; base += blockDim.x) {
+        const int64_t i = base + lane;
+        count_ids(counts, i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1, lane);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) moe_copy_kernel(const T *__restrict__ X, int64_t ldx, const int *__restrict__ slots, T *__restrict__ xs,
-                                                       int64_t ldxs, int top_k, int hidden)
+// counts[block][expert] of the block's assignments
+template <typename I>
+__global__ void __launch_bounds__(kThreads) moe_count_kernel(const I *__restrict__ ids, int experts, int count, int per_block, int *__restrict__ counts)
 {
-    const int t = blockIdx.x;
-    for (int i = threadIdx.x; i < hidden; i += blockDim.x) {
-        const T v = X[(int64_t)t * ldx + i];
-        for (int j = 0; j < top_k; ++j) {
-            const int at = slots[(int64_t)t * top_k + j];
-            if (at >= 0) xs[(int64_t)at * ldxs + i] = v;
+    extern __shared__ int mine[];
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    for (int e = threadIdx.x; e < experts; e += kThreads) mine[e] = 0;
+    __syncthreads();
+    const int64_t first = (int64_t)blockIdx.x * per_block;
+    count_range(ids, first, min((int64_t)count, first + per_block), experts, mine);
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kThreads) counts[(int64_t)blockIdx.x * experts + e] = mine[e];
+}
+
+// counts[block][expert] -> how many earlier blocks have, totals[expert]; one warp per expert
+__global__ void __launch_bounds__(kThreads) moe_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int experts, int blocks)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const int e = (int)(blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    if (e >= experts) return;
+    int sum = 0;
+    for (int base = 0; base < blocks; base += 32) {
+        const int b = base + lane;
+        const int v = b < blocks ? counts[(int64_t)b * experts + e] : 0;
+        int s = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+            if (lane >= d) s += o;
+        }
+        if (b < blocks) counts[(int64_t)b * experts + e] = sum + s - v;
+        sum += __shfl_sync(0xFFFFFFFFu, s, 31);
+    }
+    if (lane == 0) totals[e] = sum;
+}
+
+// Slots of the block's tokens and the copy of their rows.  counts == NULL: the block counts all ids itself.
+template <typename T, typename I, int VEC>
+__global__ void __launch_bounds__(kThreads) moe_place_kernel(const T *__restrict__ X, int64_t ldx, const I *__restrict__ ids, int experts, int tokens,
+                                                             int top_k, int hidden, int per_block, const int *__restrict__ counts,
+                                                             const int *__restrict__ totals, T *__restrict__ xs, int64_t ldxs, int *__restrict__ offsets,
+                                                             int *__restrict__ slots)
+{
+    extern __shared__ int smem[];
+    int *next = smem, *total = smem + experts, *at = total + experts;  // at: the slots of the block's assignments
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const int64_t first = (int64_t)blockIdx.x * per_block * top_k;
+    const int64_t last = min((int64_t)tokens * top_k, first + (int64_t)per_block * top_k);
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        next[e] = counts ? counts[(int64_t)blockIdx.x * experts + e] : 0;
+        total[e] = counts ? totals[e] : 0;
+    }
+    __syncthreads();
+    if (!counts) {
+        count_range(ids, 0, first, experts, next);
+        count_range(ids, first, (int64_t)tokens * top_k, experts, total);
+        __syncthreads();
+    }
+    if (warp == 0) {
+        // offsets: an exclusive scan of the totals; next[e] becomes the slot of the block's first assignment to e
+        int sum = 0;
+        for (int base = 0; base < experts; base += 32) {
+            const int e = base + lane;
+            const int v = e < experts ? total[e] + (counts ? 0 : next[e]) : 0;
+            int s = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                if (lane >= d) s += o;
+            }
+            if (e < experts) {
+                next[e] += sum + s - v;
+                if (blockIdx.x == 0) offsets[e] = sum + s - v;
+            }
+            sum += __shfl_sync(0xFFFFFFFFu, s, 31);
+        }
+        if (blockIdx.x == 0 && lane == 0) offsets[experts] = sum;
+        __syncwarp();
+        // the block's assignments in order, 32 at a time; lanes with the same expert are ranked by a match
+        for (int64_t base = first; base < last; base += 32) {
+            const int64_t i = base + lane;
+            const int e = i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1;
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+            const int rank = __popc(same & ((1u << lane) - 1u));
+            const int slot = e >= 0 ? next[e] + rank : -1;
+            __syncwarp();
+            if (e >= 0 && rank == 0) next[e] += __popc(same);
+            __syncwarp();
+            if (i < last) {
+                slots[i] = slot;
+                at[i - first] = slot;
+            }
         }
     }
+    __syncthreads();
+    if (hidden == 0) return;
+    const int pieces = hidden / VEC;
+    const int block_tokens = (int)((last - first) / top_k);
+    // the block's (token, piece) pairs are dealt to its threads
+    for (int64_t i = threadIdx.x; i < (int64_t)block_tokens * pieces; i += kThreads) {
+        const int t = (int)(i / pieces), c = (int)(i - (int64_t)t * pieces) * VEC;
+        Piece<T, VEC> v;
+        v.load(X + ((int64_t)blockIdx.x * per_block + t) * ldx + c);
+        for (int j = 0; j < top_k; ++j) {
+            const int slot = at[t * top_k + j];
+            if (slot >= 0) v.store(xs + (int64_t)slot * ldxs + c);
+        }
+    }
+}
+
+// y[t] = sum of weight * row; a block takes one token and a stretch of `hidden`
+template <typename T, typename S, int VEC>
+__global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restrict__ ys, int64_t ldys, int rows, const int *__restrict__ slots,
+                                                               const S *__restrict__ weights, T *__restrict__ y, int64_t ldy, int top_k, int hidden,
+                                                               int parts)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    constexpr int kAhead = 8;  // rows in flight per thread
+    const int64_t t = blockIdx.x / parts;
+    const int part = (int)(blockIdx.x % parts);
+    for (int c = (part * kThreads + (int)threadIdx.x) * VEC; c < hidden; c += parts * kThreads * VEC) {
+        float sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+        for (int j0 = 0; j0 < top_k; j0 += kAhead) {
+            Piece<T, VEC> v[kAhead];
+            float w[kAhead];
+            bool live[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                live[j] = false;
+                if (j0 + j >= top_k) continue;
+                const int at = __ldg(slots + t * top_k + j0 + j);
+                live[j] = at >= 0 && at < rows;
+                if (!live[j]) continue;
+                w[j] = weights ? to_float(__ldg(weights + t * top_k + j0 + j)) : 1.0f;
+                v[j].load(ys + (int64_t)at * ldys + c);
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (!live[j]) continue;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum[i] = fmaf(w[j], to_float(v[j].v[i]), sum[i]);
+            }
+        }
+        Piece<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = from_float<T>(sum[i]);
+        o.store(y + t * ldy + c);
+    }
+}
+
+// Both gradients of one token: dy is read once, every row of ys once, every row of dys is written once; the products with the
+// rows are summed over the block in a fixed order.
+template <typename T, typename S, int VEC>
+__global__ void __launch_bounds__(kThreads) moe_combine_grad_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ ys, int64_t ldys, int rows,
+                                                                    const int *__restrict__ slots, const S *__restrict__ weights, T *__restrict__ dys,
+                                                                    int64_t lddys, S *__restrict__ dweights, int top_k, int hidden)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    constexpr int kAhead = 4;
+    __shared__ float part[kThreads / 32][kAhead];
+    const int64_t t = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int j0 = 0; j0 < top_k; j0 += kAhead) {
+        int at[kAhead];
+        float w[kAhead], dot[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            at[j] = j0 + j < top_k ? __ldg(slots + t * top_k + j0 + j) : -1;
+            if (at[j] >= rows) at[j] = -1;
+            w[j] = at[j] >= 0 ? to_float(__ldg(weights + t * top_k + j0 + j)) : 0.0f;
+            dot[j] = 0.0f;
+        }
+        for (int c = (int)threadIdx.x * VEC; c < hidden; c += kThreads * VEC) {
+            Piece<T, VEC> d, v[kAhead];
+            d.load(dy + t * lddy + c);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (at[j] >= 0) v[j].load(ys + (int64_t)at[j] * ldys + c);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (at[j] < 0) continue;
+                Piece<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float g = to_float(d.v[i]);
+                    dot[j] = fmaf(g, to_float(v[j].v[i]), dot[j]);
+                    o.v[i] = from_float<T>(w[j] * g);
+                }
+                o.store(dys + (int64_t)at[j] * lddys + c);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+            for (int s = 16; s; s >>= 1) dot[j] += __shfl_xor_sync(0xFFFFFFFFu, dot[j], s);
+            if (lane == 0) part[warp][j] = dot[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < kAhead && j0 + (int)threadIdx.x < top_k) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kThreads / 32; ++k) sum += part[k][threadIdx.x];
+            dweights[t * top_k + j0 + threadIdx.x] = from_float<S>(sum);
+        }
+        __syncthreads();
+    }
+}
+
+bool on16(const void *p, int64_t pitch, int size) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (pitch * size) % 16 == 0; }
+
+// f gets the piece width: 16 bytes where `vec`, else one element
+template <typename T, typename F>
+int with_pieces(bool vec, F f)
+{
+    return vec ? f(std::integral_constant<int, 16 / (int)sizeof(T)>()) : f(std::integral_constant<int, 1>());
+}
+
+constexpr int kMaxSlots = 8192;  // slots a block keeps in shared memory; top_k is at most half of it
+
+int tokens_per_block(int tokens, int top_k)
+{
+    const int per = (tokens + kBlocks - 1) / kBlocks, most = kMaxSlots / (top_k > 0 ? top_k : 1);
+    return per < 1 ? 1 : per < most ? per : most;
+}
+
+}  // namespace
+
+size_t moe_sort_workspace(int tokens, int top_k, int experts)
+{
+    if ((int64_t)tokens * top_k <= kFewIds) return 0;
+    const int per = tokens_per_block(tokens, top_k), blocks = (tokens + per - 1) / per;
+    return ((size_t)blocks + 1) * experts * sizeof(int);
 }
 
 int moe_sort_launch(const MoeSortArgs &a)
 {
+    const int per = tokens_per_block(a.tokens, a.top_k), blocks = a.tokens > 0 ? (a.tokens + per - 1) / per : 1;
     const int count = a.tokens * a.top_k;
-    const size_t smem = ((size_t)a.experts + 1) * sizeof(int);
-    if (a.id_bytes == 8)
-        moe_slots_kernel<int64_t><<<1, 1024, smem, a.stream>>>(static_cast<const int64_t *>(a.ids), a.experts, count, a.offsets, a.slots);
-    else
-        moe_slots_kernel<int32_t><<<1, 1024, smem, a.stream>>>(static_cast<const int32_t *>(a.ids), a.experts, count, a.offsets, a.slots);
-    int st = launched("moe_slots_kernel launch");
-    if (st != QM_OK || count == 0 || a.hidden == 0) return st;
-    return with_type(a.type, [&](auto t) {
-        using T = typename decltype(t)::type;
-        moe_copy_kernel<T><<<(unsigned)a.tokens, 256, 0, a.stream>>>(static_cast<const T *>(a.X), a.ldx, a.slots, static_cast<T *>(a.xs), a.ldxs, a.top_k,
-                                                                     a.hidden);
-        return launched("moe_copy_kernel launch");
-    });
-}
-
-template <typename T, typename S>
-__global__ void __launch_bounds__(256) moe_combine_kernel(const T *__restrict__ ys, int64_t ldys, int rows, const int *__restrict__ slots,
-                                                          const S *__restrict__ weights, T *__restrict__ y, int64_t ldy, int top_k, int hidden)
-{
-    const int64_t t = blockIdx.x;
-    for (int i = threadIdx.x; i < hidden; i += blockDim.x) {
-        float sum = 0.0f;
-        for (int j = 0; j < top_k; ++j) {
-            const int at = slots[t * top_k + j];
-            if (at < 0 || at >= rows) continue;
-            sum = fmaf(weights ? to_float(weights[t * top_k + j]) : 1.0f, to_float(ys[(int64_t)at * ldys + i]), sum);
+    const size_t smem = ((size_t)2 * a.experts + (size_t)per * a.top_k) * sizeof(int);
+    int *counts = nullptr, *totals = nullptr;
+    auto by_id = [&](auto id) {
+        using I = typename decltype(id)::type;
+        const I *ids = static_cast<const I *>(a.ids);
+        if (count > kFewIds) {
+            totals = a.workspace;
+            counts = a.workspace + a.experts;
+            int st = launch_chained("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kThreads, (size_t)a.experts * sizeof(int), a.stream, ids,
+                                    a.experts, count, per * a.top_k, counts);
+            if (st != QM_OK) return st;
+            st = launch_chained("moe_scan_kernel launch", moe_scan_kernel, (unsigned)((a.experts + 7) / 8), kThreads, 0, a.stream, counts, totals, a.experts,
+                                blocks);
+            if (st != QM_OK) return st;
         }
-        y[t * ldy + i] = from_float<T>(sum);
-    }
-}
-
-template <typename T, typename S>
-__global__ void __launch_bounds__(256) moe_combine_grad_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ ys, int64_t ldys, int rows,
-                                                               const int *__restrict__ slots, const S *__restrict__ weights, T *__restrict__ dys,
-                                                               int64_t lddys, S *__restrict__ dweights, int top_k, int hidden)
-{
-    __shared__ float part[8];
-    const int64_t i = blockIdx.x, t = i / top_k;  // one assignment per block
-    const int at = slots[i];
-    if (at < 0 || at >= rows) {
-        if (threadIdx.x == 0) dweights[i] = from_float<S>(0.0f);
-        return;
-    }
-    const float w = to_float(weights[i]);
-    float dot = 0.0f;
-    for (int c = threadIdx.x; c < hidden; c += blockDim.x) {
-        const float d = to_float(dy[t * lddy + c]);
-        dot = fmaf(d, to_float(ys[(int64_t)at * ldys + c]), dot);
-        dys[(int64_t)at * lddys + c] = from_float<T>(w * d);
-    }
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, d);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float sum = 0.0f;
-        for (int k = 0; k < 8; ++k) sum += part[k];
-        dweights[i] = from_float<S>(sum);
-    }
+        return with_type(a.type, [&](auto t) {
+            using T = typename decltype(t)::type;
+            const bool vec = on16(a.X, a.ldx, sizeof(T)) && on16(a.xs, a.ldxs, sizeof(T)) && a.hidden % (16 / (int)sizeof(T)) == 0;
+            return with_pieces<T>(vec, [&](auto v) {
+                constexpr int VEC = decltype(v)::value;
+                auto kernel = moe_place_kernel<T, I, VEC>;
+                if (smem > 48 * 1024) {
+                    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                    if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(moe_place_kernel)");
+                }
+                return launch_chained("moe_place_kernel launch", kernel, (unsigned)blocks, kThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
+                                      a.experts, a.tokens, a.top_k, a.hidden, per, (const int *)counts, (const int *)totals, static_cast<T *>(a.xs), a.ldxs,
+                                      a.offsets, a.slots);
+            });
+        });
+    };
+    return a.id_bytes == 8 ? by_id(Tag<int64_t>()) : by_id(Tag<int32_t>());
 }
 
 int moe_combine_launch(const MoeCombineArgs &a)
@@ -125,10 +342,16 @@ int moe_combine_launch(const MoeCombineArgs &a)
         using T = typename decltype(t)::type;
         return with_same_or_float<T>(a.weight_type, [&](auto u) {
             using S = typename decltype(u)::type;
-            moe_combine_kernel<T, S><<<(unsigned)a.tokens, 256, 0, a.stream>>>(static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots,
-                                                                               static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo, a.top_k,
-                                                                               a.hidden);
-            return launched("moe_combine_kernel launch");
+            const bool vec = on16(a.ys, a.ldys, sizeof(T)) && on16(a.out, a.ldo, sizeof(T)) && a.hidden % (16 / (int)sizeof(T)) == 0;
+            return with_pieces<T>(vec, [&](auto v) {
+                constexpr int VEC = decltype(v)::value;
+                // a thread per piece while the grid allows it
+                int64_t parts = (a.hidden + kThreads * VEC - 1) / (kThreads * VEC);
+                if (parts * a.tokens > 0x7FFFFFFF) parts = 1;
+                return launch_chained("moe_combine_kernel launch", moe_combine_kernel<T, S, VEC>, (unsigned)(parts * a.tokens), kThreads, 0, a.stream,
+                                      static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots, static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo,
+                                      a.top_k, a.hidden, (int)parts);
+            });
         });
     });
 }
@@ -139,10 +362,14 @@ int moe_combine_grad_launch(const MoeCombineArgs &a)
         using T = typename decltype(t)::type;
         return with_same_or_float<T>(a.weight_type, [&](auto u) {
             using S = typename decltype(u)::type;
-            moe_combine_grad_kernel<T, S><<<(unsigned)(a.tokens * a.top_k), 256, 0, a.stream>>>(
-                static_cast<const T *>(a.dy), a.lddy, static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots, static_cast<const S *>(a.weights),
-                static_cast<T *>(a.out), a.ldo, static_cast<S *>(a.dweights), a.top_k, a.hidden);
-            return launched("moe_combine_grad_kernel launch");
+            const bool vec = on16(a.dy, a.lddy, sizeof(T)) && on16(a.ys, a.ldys, sizeof(T)) && on16(a.out, a.ldo, sizeof(T)) &&
+                             a.hidden % (16 / (int)sizeof(T)) == 0;
+            return with_pieces<T>(vec, [&](auto v) {
+                constexpr int VEC = decltype(v)::value;
+                return launch_chained("moe_combine_grad_kernel launch", moe_combine_grad_kernel<T, S, VEC>, (unsigned)a.tokens, kThreads, 0, a.stream,
+                                      static_cast<const T *>(a.dy), a.lddy, static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots,
+                                      static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo, static_cast<S *>(a.dweights), a.top_k, a.hidden);
+            });
         });
     });
 }

@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstdlib>
+
 #include "qm_internal.h"
 
 namespace qm {
@@ -46,6 +48,26 @@ template <typename T, typename F>
 int with_same_or_float(int other, F f)
 {
     return other == QM_TYPE_F32 ? f(Tag<float>()) : f(Tag<T>());
+}
+
+// Launch that may begin while the previous kernel of the stream still runs: the kernel waits (griddepcontrol.wait) before it
+// touches global memory.  QM_NO_PDL=1 turns that off.
+template <typename... P, typename... A>
+int launch_chained(const char *what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t stream, A... args)
+{
+    static const bool allow = !std::getenv("QM_NO_PDL");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = allow ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
 }
 
 inline int launched(const char *what)

@@ -1,34 +1,137 @@
 // Group-wise 4-bit quantiser: per group of a row, scale = max |w| times the fp32 value of 1/7 (rounded to the scales' type) and
 // code = w / scale, the exact quotient rounded to the nearest integer, ties to even.
+//
+// Bound by memory: every element is read once and leaves as half a byte.  A lane takes eight consecutive elements (one or two
+// 16-byte loads) and writes their four bytes; 4, 8, 16 or 32 neighbouring lanes share a group, whose maximum is a few shuffles.
+// A warp has kUnroll such pieces of 256 elements in flight.
+#include <cstdlib>
+
+#include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
 namespace qm {
 
 using namespace w4;
 
-// The code of w for scale s.  q = w * (1 / s) rounded is off by at most one; the remainder w - q s is exact in one fma (w and q s
-// are multiples of the smaller of their last places and the result has at most 24 bits: for |q| >= 2 it is at most s and a
-// multiple of s's last place, for |q| = 1 it is a difference of numbers within a factor of two), so comparing it with s / 2
-// finds the nearest integer and the ties.
-__device__ __forceinline__ int code_of(float w, float s, float inv)
+namespace {
+
+constexpr int kThreads = 256, kUnroll = 4;
+
+// Scale and reciprocal for a group with largest value a, ready for code_of: both sides of the quotient are multiplied by `up`, 2^64
+// for scales near or below the smallest normal number, which have no reciprocal.  some = false: the codes are 0.
+struct Quotient {
+    float s, inv, up;
+    bool some;
+};
+
+template <typename S>
+__device__ __forceinline__ Quotient quotient_for(S stored)
 {
-    float q = rintf(w * inv);
-    const float r = fmaf(-q, s, w), half = 0.5f * s;
-    if (r > half || (r == half && ((int)q & 1))) q += 1.0f;
-    else if (r < -half || (r == -half && ((int)q & 1))) q -= 1.0f;
-    return (int)fminf(fmaxf(q, -8.0f), 7.0f);
+    Quotient q;
+    q.s = to_float(stored);
+    q.some = q.s > 0.0f && q.s < INFINITY;
+    q.up = q.s < 0x1p-100f ? 0x1p64f : 1.0f;
+    q.s *= q.up;
+    q.inv = q.some ? __frcp_rn(q.s) : 0.0f;
+    return q;
 }
 
-// One warp per group, whatever the group's width.
-template <typename T, typename S>
-__global__ void __launch_bounds__(256) quantize_w4_kernel(const T *__restrict__ W, int64_t ldw, uint8_t *__restrict__ packed, S *__restrict__ scales,
-                                                          int64_t rows, int64_t k, int group)
+// The code of w.  q = w * (1 / s) rounded is off by at most one; the remainder w - q s is exact in one fma (w and q s are multiples
+// of the smaller of their last places and the result has at most 24 bits: for |q| >= 2 it is at most s and a multiple of s's last
+// place, for |q| = 1 it is a difference of numbers within a factor of two), so comparing it with s / 2 finds the nearest
+// integer and the ties.
+__device__ __forceinline__ int code_of(float w, const Quotient &z)
 {
+    w *= z.up;
+    const float q = rintf(w * z.inv);
+    const float r = fmaf(-q, z.s, w), half = 0.5f * z.s;
+    int n = (int)q;  // |w| is at most a few scales, or the group has no codes
+    const bool odd = (n & 1) != 0;
+    if (r > half || (r == half && odd)) n += 1;
+    if (r < -half || (r == -half && odd)) n -= 1;
+    return min(max(n, -8), 7);
+}
+
+// Eight elements from 16-byte loads.
+template <typename T>
+struct Eight {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ float at(int i) const { return to_float(reinterpret_cast<const T *>(v)[i]); }
+};
+
+// k % 8 == 0 and rows on 16-byte boundaries.  Pieces of 256 elements are dealt to the warps.
+template <typename T, typename S>
+__global__ void __launch_bounds__(kThreads) quantize_w4_kernel(const T *__restrict__ W, int64_t ldw, uint8_t *__restrict__ packed, S *__restrict__ scales,
+                                                               int64_t rows, int k, int group_shift)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const int lanes = 1 << (group_shift - 3);  // lanes that share a group
+    const int per_row = (k + 255) / 256, groups = (k + (1 << group_shift) - 1) >> group_shift;
+    const int64_t pieces = rows * per_row, stride = (int64_t)gridDim.x * (kThreads / 32);
+    for (int64_t first = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); first < pieces; first += stride * kUnroll) {
+        Eight<T> w[kUnroll];
+        int64_t row[kUnroll];
+        int at[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t i = first + u * stride;
+            row[u] = i / per_row;
+            at[u] = (int)(i - row[u] * per_row) * 256 + lane * 8;
+            if (i >= pieces) at[u] = k;
+            if (at[u] < k) w[u].load(W + row[u] * ldw + at[u]);
+            else w[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float a = 0.0f, bad = 0.0f;  // bad becomes NaN with any NaN: max drops them
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = w[u].at(j);
+                a = fmaxf(a, fabsf(v));
+                bad = v != v ? v : bad;
+            }
+            unsigned nan = __ballot_sync(0xFFFFFFFFu, bad != bad);
+            for (int d = 1; d < lanes; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, d));
+            nan &= (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (lane & ~(lanes - 1));
+            if (nan) a = __int_as_float(0x7FC00000);
+            const S stored = from_float<S>(__fmul_rn(a, 1.0f / 7.0f));
+            const Quotient z = quotient_for(stored);
+            uint32_t word = 0;
+            if (z.some) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) word |= (uint32_t)(code_of(w[u].at(j), z) & 15) << (4 * j);
+            }
+            if (at[u] < k) {
+                __stcs(reinterpret_cast<uint32_t *>(packed + row[u] * (k / 2) + at[u] / 2), word);
+                if ((lane & (lanes - 1)) == 0) scales[row[u] * groups + (at[u] >> group_shift)] = stored;
+            }
+        }
+    }
+}
+
+// Any even k and any alignment: one warp per group.
+template <typename T, typename S>
+__global__ void __launch_bounds__(kThreads) quantize_w4_any_kernel(const T *__restrict__ W, int64_t ldw, uint8_t *__restrict__ packed,
+                                                                   S *__restrict__ scales, int64_t rows, int64_t k, int group)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int64_t groups = (k + group - 1) / group;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows * groups; i += (int64_t)gridDim.x * 8) {
-        const int64_t row = i / groups, g = i - row * groups;
-        const int64_t first = g * group, last = min(k, first + group);
+    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < rows * groups; i += (int64_t)gridDim.x * (kThreads / 32)) {
+        const int64_t row = i / groups, first = (i - row * groups) * group, last = min(k, first + group);
         const T *w = W + row * ldw;
         float a = 0.0f;
         bool nan = false;
@@ -41,21 +144,16 @@ __global__ void __launch_bounds__(256) quantize_w4_kernel(const T *__restrict__ 
         if (__any_sync(0xFFFFFFFFu, nan)) a = __int_as_float(0x7FC00000);
         const S stored = from_float<S>(__fmul_rn(a, 1.0f / 7.0f));
         if (lane == 0) scales[i] = stored;
-        float s = to_float(stored);
-        const bool some = s > 0.0f && s < INFINITY;
-        // a scale near or below the smallest normal number has no reciprocal: both sides of the quotient times 2^64, exactly
-        const float up = s < 0x1p-100f ? 0x1p64f : 1.0f;
-        s *= up;
+        const Quotient z = quotient_for(stored);
         for (int64_t j = first + 2 * lane; j < last; j += 64) {
             int low = 0, high = 0;
-            if (some) {
-                low = code_of(to_float(w[j]) * up, s, 1.0f / s);
-                high = code_of(to_float(w[j + 1]) * up, s, 1.0f / s);
-            }
+            if (z.some) low = code_of(to_float(w[j]), z), high = code_of(to_float(w[j + 1]), z);
             packed[row * (k / 2) + j / 2] = (uint8_t)((low & 15) | (high << 4));
         }
     }
 }
+
+}  // namespace
 
 int quantize_w4_launch(const void *W, int type, int64_t ldw, uint8_t *packed, void *scales, int scale_type, int64_t rows, int64_t k, int group,
                        cudaStream_t stream)
@@ -64,10 +162,18 @@ int quantize_w4_launch(const void *W, int type, int64_t ldw, uint8_t *packed, vo
         using T = typename decltype(t)::type;
         return with_same_or_float<T>(scale_type, [&](auto u) {
             using S = typename decltype(u)::type;
+            const T *w = static_cast<const T *>(W);
+            S *s = static_cast<S *>(scales);
+            const bool vec = k % 8 == 0 && k < (1 << 30) && (reinterpret_cast<uintptr_t>(W) & 15u) == 0 && (ldw * (int64_t)sizeof(T)) % 16 == 0 &&
+                             (reinterpret_cast<uintptr_t>(packed) & 3u) == 0;
+            if (vec) {
+                const int64_t pieces = rows * ((k + 255) / 256), blocks = (pieces + 8 * kUnroll - 1) / (8 * kUnroll);
+                return launch_chained("quantize_w4_kernel launch", quantize_w4_kernel<T, S>, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), kThreads, 0,
+                                      stream, w, ldw, packed, s, rows, (int)k, group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8);
+            }
             const int64_t blocks = (rows * ((k + group - 1) / group) + 7) / 8;
-            quantize_w4_kernel<T, S><<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream>>>(static_cast<const T *>(W), ldw, packed,
-                                                                                                        static_cast<S *>(scales), rows, k, group);
-            return launched("quantize_w4_kernel launch");
+            return launch_chained("quantize_w4_any_kernel launch", quantize_w4_any_kernel<T, S>, (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), kThreads,
+                                  0, stream, w, ldw, packed, s, rows, k, group);
         });
     });
 }

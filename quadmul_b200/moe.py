@@ -9,9 +9,9 @@ The reference has no counterpart.  Everything is deterministic: there are no flo
 """
 from __future__ import annotations
 
-from . import _count, _on_device, _stream_of, _torch
+from . import _EXT, _count, _on_device, _stream_of, _torch
 from ._lib import LIB, check
-from .w4 import check_out, check_rows, check_whole, moe_gemm_w4, pitch, type_of
+from .w4 import check_out, check_rows, check_whole, compiled, moe_gemm_w4, pitch, type_of
 
 MAX_EXPERTS = 4096
 
@@ -41,6 +41,10 @@ def moe_sort(x, expert_ids, num_experts: int, out=None):
     `out` (and undefined in an xs that is allocated here)."""
     what = "moe_sort"
     torch = _torch()
+    if _EXT is not None:
+        result = compiled(_EXT.moe_sort, x, expert_ids, num_experts, out)
+        _count(3 if LIB.qm_moe_sort_workspace_bytes(*expert_ids.shape, num_experts) else 1)
+        return result
     code = type_of(what, "x", x)
     check_rows(what, x=x)
     check_whole(what, x.device, expert_ids=expert_ids)
@@ -51,14 +55,19 @@ def moe_sort(x, expert_ids, num_experts: int, out=None):
     if not 0 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"{what}: num_experts must be within [0, {MAX_EXPERTS}]")
     (tokens, hidden), top_k = x.shape, expert_ids.shape[1]
+    if top_k > MAX_EXPERTS or tokens * top_k >= 1 << 31:
+        raise ValueError(f"{what}: too many assignments")
     xs = check_out(what, "out", out, (tokens * top_k, hidden), x)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=x.device)
     slots = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
+    need = LIB.qm_moe_sort_workspace_bytes(tokens, top_k, num_experts)
+    workspace = torch.empty(need // 4, dtype=torch.int32, device=x.device) if need else None
     with _on_device(x):
         st = LIB.qm_moe_sort(x.data_ptr(), code, pitch(x), expert_ids.data_ptr(), expert_ids.element_size(), num_experts, xs.data_ptr(), pitch(xs),
-                             offsets.data_ptr(), slots.data_ptr(), tokens, top_k, hidden, _stream_of(x))
+                             offsets.data_ptr(), slots.data_ptr(), tokens, top_k, hidden, None if workspace is None else workspace.data_ptr(),
+                             need, _stream_of(x))
     check(st, f"{what}(tokens={tokens}, top_k={top_k}, hidden={hidden}, experts={num_experts})")
-    _count(2)
+    _count(3 if need else 1)
     return xs, offsets, slots
 
 
@@ -68,6 +77,9 @@ def moe_combine(ys, slots, weights=None, out=None):
     ys [rows, hidden]; slots int32 [tokens, top_k] as `moe_sort` returns them (a slot outside [0, rows) adds nothing, a token
     without any gets zeros); weights [tokens, top_k] of ys's type or float32, None for all ones."""
     what = "moe_combine"
+    if _EXT is not None:
+        _count(1)
+        return compiled(_EXT.moe_combine, ys, slots, weights, out)
     code = type_of(what, "ys", ys)
     check_rows(what, ys=ys)
     _check_slots(what, slots, ys.device)
@@ -94,6 +106,9 @@ def moe_combine_grad(dy, ys, slots, weights, out=None):
     The slots within [0, rows) must differ from one another, as those of `moe_sort` do.  Rows of dys that no slot names are left
     as they were in `out` (and undefined in a dys that is allocated here)."""
     what = "moe_combine_grad"
+    if _EXT is not None:
+        _count(1)
+        return compiled(_EXT.moe_combine_grad, dy, ys, slots, weights, out)
     torch = _torch()
     code = type_of(what, "dy", dy)
     if type_of(what, "ys", ys) != code:

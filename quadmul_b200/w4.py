@@ -9,10 +9,18 @@ products are not recorded by autograd: an input that requires a gradient is refu
 """
 from __future__ import annotations
 
-from . import _count, _on_device, _stream_of, _torch
-from ._lib import LIB, QM_TYPE_BF16, QM_TYPE_F16, QM_TYPE_F32, check
+from . import _EXT, _count, _on_device, _stream_of, _torch
+from ._lib import LIB, QM_TYPE_BF16, QM_TYPE_F16, QM_TYPE_F32, QuadmulError, check
 
 GROUPS = (32, 64, 128, 256)
+
+
+def compiled(call, *args):
+    """A call of the compiled binding, which checks as the ctypes form does; its status errors become QuadmulError."""
+    try:
+        return call(*args)
+    except RuntimeError as exc:
+        raise QuadmulError(-1, str(exc).split("\n")[0]) from exc
 
 
 def type_of(what: str, name: str, t, allowed=None) -> int:
@@ -98,6 +106,9 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
     `quantize_w4` write them; scales [n, ceil(k / group)]: x's type or float32; group: 32, 64, 128 or 256.  Returns out, of x's
     type (allocated when not passed in).  Asynchronous on the current stream of x's device."""
     what = "gemm_w4"
+    if _EXT is not None:
+        _count(1)
+        return compiled(_EXT.gemm_w4, x, b, scales, group, out)
     code, scode, n, k = _check_weights(what, x, b, scales, group, ())
     m = x.shape[0]
     out = check_out(what, "out", out, (m, n), x)
@@ -116,6 +127,9 @@ def moe_gemm_w4(x, b, scales, offsets, group: int = 128, out=None):
     [experts + 1] on the device, as `moe_sort` returns them.  Rows that belong to no expert are left as they were in `out` (and
     undefined in an `out` that is allocated here).  The launch does not depend on the values of offsets."""
     what = "moe_gemm_w4"
+    if _EXT is not None:
+        _count(1)
+        return compiled(_EXT.moe_gemm_w4, x, b, scales, offsets, group, out)
     torch = _torch()
     if b.dim() != 3:
         raise ValueError(f"{what}: b must be [experts, n, k/2]")
@@ -142,6 +156,12 @@ def quantize_w4(w, group: int = 128, scale_dtype=None):
     has a scale that is not finite and codes 0."""
     what = "quantize_w4"
     torch = _torch()
+    scale_dtype = w.dtype if scale_dtype is None else scale_dtype
+    if scale_dtype not in (w.dtype, torch.float32):
+        raise TypeError(f"{what}: scale_dtype must be {w.dtype} or torch.float32")
+    if _EXT is not None:
+        _count(1)
+        return compiled(_EXT.quantize_w4, w, group, scale_dtype == torch.float32)
     code = type_of(what, "w", w)
     check_rows(what, w=w)
     if group not in GROUPS:
@@ -149,9 +169,6 @@ def quantize_w4(w, group: int = 128, scale_dtype=None):
     n, k = w.shape
     if k % 2:
         raise ValueError(f"{what}: k must be even")
-    scale_dtype = w.dtype if scale_dtype is None else scale_dtype
-    if scale_dtype not in (w.dtype, torch.float32):
-        raise TypeError(f"{what}: scale_dtype must be {w.dtype} or torch.float32")
     packed = torch.empty((n, k // 2), dtype=torch.int8, device=w.device)
     scales = torch.empty((n, -(-k // group)), dtype=scale_dtype, device=w.device)
     with _on_device(w):

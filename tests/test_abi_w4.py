@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 F32, F16, BF16 = 0, 1, 2
-NULL_, SHAPE, ALIGN, ARG = 1, 2, 3, 8
+NULL_, SHAPE, ALIGN, WORKSPACE, ARG = 1, 2, 3, 7, 8
 
 
 @pytest.fixture()
@@ -58,12 +58,14 @@ def test_quantize_w4(lib, p):
 
 def test_moe_sort(lib, p):
     def call(X=p, type=F32, ldx=8, ids=p, id_bytes=8, experts=4, xs=p, ldxs=8, offsets=p, slots=p, tokens=2, top_k=2, hidden=8):
-        return lib.qm_moe_sort(X, type, ldx, ids, id_bytes, experts, xs, ldxs, offsets, slots, tokens, top_k, hidden, None)
+        return lib.qm_moe_sort(X, type, ldx, ids, id_bytes, experts, xs, ldxs, offsets, slots, tokens, top_k, hidden, None, 0, None)
 
     assert call(tokens=-1) == SHAPE and call(top_k=-1) == SHAPE and call(hidden=-1) == SHAPE and call(experts=-1) == SHAPE and call(experts=4097) == SHAPE
-    assert call(tokens=1 << 20, top_k=1 << 12) == SHAPE and call(ldx=7) == SHAPE and call(ldxs=7) == SHAPE
+    assert call(tokens=1 << 20, top_k=1 << 12) == SHAPE and call(top_k=4097) == SHAPE and call(ldx=7) == SHAPE and call(ldxs=7) == SHAPE
     assert call(type=4) == ARG and call(id_bytes=2) == ARG
     assert call(offsets=None) == NULL_ and call(slots=None) == NULL_ and call(ids=None) == NULL_ and call(X=None) == NULL_ and call(xs=None) == NULL_
+    assert lib.qm_moe_sort_workspace_bytes(16, 8, 64) == 0 and lib.qm_moe_sort_workspace_bytes(1 << 15, 8, 64) > 0
+    assert call(tokens=1 << 15, top_k=8) == WORKSPACE
     assert call(offsets=p + 1) == ALIGN and call(slots=p + 2) == ALIGN and call(ids=p + 4) == ALIGN and call(X=p + 2) == ALIGN and call(xs=p + 2) == ALIGN
 
 

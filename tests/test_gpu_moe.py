@@ -259,7 +259,35 @@ def test_a_feed_forward_layer_of_experts(qm, cuda_clean, tokens):
     assert float((y.double() - want).norm() / want.norm()) <= 6 * HALF_STEP[BF16]
 
 
-def test_refusals(qm, cuda_clean):
+@pytest.fixture(params=["compiled", "ctypes"])
+def binding(request, monkeypatch):
+    """Both ways into the library: the compiled binding, and the ctypes form that is used without it."""
+    import quadmul_b200.moe
+    import quadmul_b200.w4
+
+    if request.param == "ctypes":
+        monkeypatch.setattr(quadmul_b200.w4, "_EXT", None)
+        monkeypatch.setattr(quadmul_b200.moe, "_EXT", None)
+    elif quadmul_b200.w4._EXT is None:
+        pytest.skip("the compiled binding is not built")
+
+
+@pytest.mark.parametrize("tokens", [40, 5000])
+def test_both_bindings(qm, cuda_clean, binding, tokens):
+    top_k, experts, hidden = 4, 9, 24
+    ids = routing(tokens, top_k, experts, 0.1, 1)
+    offsets, slots = order(ids, experts)
+    x = torch.randn(tokens, hidden, generator=torch.Generator().manual_seed(2))
+    xs, got_offsets, got_slots = qm.moe_sort(x.cuda(), ids.cuda(), experts)
+    assert torch.equal(got_offsets.cpu(), offsets) and torch.equal(got_slots.cpu(), slots)
+    w = torch.ones(tokens, top_k).cuda()
+    assert torch.equal(qm.moe_combine(xs, got_slots, w), qm.moe_sort_grad(xs, got_slots))
+    dys, dw = qm.moe_combine_grad(x.cuda(), xs, got_slots, w)
+    last = int(offsets[-1])
+    assert torch.equal(dys[:last], xs[:last]) and dw.shape == w.shape
+
+
+def test_refusals(qm, cuda_clean, binding):
     x, ids = torch.zeros(4, 8, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda")
     for args, error in [((x.double(), ids, 3), TypeError), ((x.int(), ids, 3), TypeError), ((x, ids.float(), 3), TypeError), ((x, ids[:3], 3), ValueError),
                         ((x, ids[:, 0], 3), ValueError), ((x, ids, -1), ValueError), ((x, ids, 4097), ValueError), ((x.cpu(), ids, 3), ValueError),

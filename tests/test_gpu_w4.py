@@ -316,7 +316,32 @@ def test_quantised_weights_in_a_product(qm, cuda_clean):
 # ---- refusals --------------------------------------------------------------------------------------------------------------
 
 
-def test_refusals(qm, cuda_clean):
+@pytest.fixture(params=["compiled", "ctypes"])
+def binding(request, monkeypatch):
+    """Both ways into the library: the compiled binding, and the ctypes form that is used without it."""
+    import quadmul_b200.moe
+    import quadmul_b200.w4
+
+    if request.param == "ctypes":
+        monkeypatch.setattr(quadmul_b200.w4, "_EXT", None)
+        monkeypatch.setattr(quadmul_b200.moe, "_EXT", None)
+    elif quadmul_b200.w4._EXT is None:
+        pytest.skip("the compiled binding is not built")
+
+
+def test_both_bindings(qm, cuda_clean, binding):
+    x, q, packed, scales = whole_case(9, 40, 128, 64, BF16, FP32, 30)
+    want = (x.double() @ dequantised(q, scales, 64).T).to(BF16)
+    assert torch.equal(run(qm, x, packed, scales, 64).cpu(), want)
+    offsets = torch.tensor([0, 4, 9], dtype=torch.int32).cuda()
+    two = (torch.stack([packed, packed]).cuda(), torch.stack([scales, scales]).cuda())
+    assert torch.equal(qm.moe_gemm_w4(x.cuda(), *two, offsets, 64).cpu(), want)
+    codes_, s = quantiser_reference(x.float(), 64, FP32)
+    p, got = qm.quantize_w4(x.cuda(), 64, scale_dtype=FP32)
+    assert torch.equal(got.cpu(), s) and torch.equal(qm.unpack(p).cpu(), codes_)
+
+
+def test_refusals(qm, cuda_clean, binding):
     def make(m=4, n=8, k=64, dtype=BF16, group=64):
         return [torch.zeros(m, k, dtype=dtype, device="cuda"), torch.zeros(n, k // 2, dtype=torch.int8, device="cuda"),
                 torch.zeros(n, -(-k // group), dtype=dtype, device="cuda"), group]
