@@ -4,8 +4,8 @@
 //
 // Sorting.  slot(t, j) = (assignments to lower experts) + (earlier assignments to the same expert): a counting sort, stable, without
 // atomics on anything that decides an order.  Up to kFewIds assignments take ONE launch: every block counts all ids itself
-// (they are L2 hits), which costs a microsecond or two and saves two launches and a workspace.  More take three: counts per
-// block of assignments, a scan of the counts over the blocks, and the placing.
+// (they are L2 hits), which saves two launches and a workspace.  More take three: counts per block of assignments, a scan of
+// the counts over the blocks, and the placing.
 #include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
@@ -16,7 +16,7 @@ using namespace w4;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kFewIds = 16384;
+constexpr int kFewIds = 2048;
 constexpr int kBlocks = 148 * 4;  // blocks that share the assignments
 
 // VEC elements of T that move together: 16 bytes, or one element where rows are not on 16-byte boundaries.
@@ -50,9 +50,16 @@ template <typename I>
 __device__ __forceinline__ void count_range(const I *__restrict__ ids, int64_t first, int64_t last, int experts, int *counts)
 {
     const int lane = threadIdx.x & 31;
-    for (int64_t base = first + (threadIdx.x & ~31); base < last; base += blockDim.x) {
-        const int64_t i = base + lane;
-        count_ids(counts, i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1, lane);
+    constexpr int kAhead = 4;  // loads in flight
+    for (int64_t base = first + (threadIdx.x & ~31); base < last; base += kAhead * (int64_t)blockDim.x) {
+        int e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t i = base + u * (int64_t)blockDim.x + lane;
+            e[u] = i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) count_ids(counts, e[u], lane);
     }
 }
 
@@ -157,15 +164,28 @@ __global__ void __launch_bounds__(kThreads) moe_place_kernel(const T *__restrict
     __syncthreads();
     if (hidden == 0) return;
     const int pieces = hidden / VEC;
-    const int block_tokens = (int)((last - first) / top_k);
+    const int block_tokens = top_k > 0 ? (int)((last - first) / top_k) : 0;
     // the block's (token, piece) pairs are dealt to its threads
-    for (int64_t i = threadIdx.x; i < (int64_t)block_tokens * pieces; i += kThreads) {
-        const int t = (int)(i / pieces), c = (int)(i - (int64_t)t * pieces) * VEC;
-        Piece<T, VEC> v;
-        v.load(X + ((int64_t)blockIdx.x * per_block + t) * ldx + c);
-        for (int j = 0; j < top_k; ++j) {
-            const int slot = at[t * top_k + j];
-            if (slot >= 0) v.store(xs + (int64_t)slot * ldxs + c);
+    constexpr int kAhead = 4;
+    const int todo = block_tokens * pieces;  // at most kMaxSlots tokens
+    for (int base = threadIdx.x; base < todo; base += kAhead * kThreads) {
+        Piece<T, VEC> v[kAhead];
+        int t[kAhead], c[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = base + u * kThreads;
+            t[u] = i < todo ? i / pieces : -1;
+            if (t[u] < 0) continue;
+            c[u] = (i - t[u] * pieces) * VEC;
+            v[u].load(X + ((int64_t)blockIdx.x * per_block + t[u]) * ldx + c[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (t[u] < 0) continue;
+            for (int j = 0; j < top_k; ++j) {
+                const int slot = at[t[u] * top_k + j];
+                if (slot >= 0) v[u].store(xs + (int64_t)slot * ldxs + c[u]);
+            }
         }
     }
 }

@@ -139,14 +139,25 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, Tag
     return r;
 }
 
-// Eight codes e0 .. e7 of one word -> four pairs (e0, e4), (e1, e5), (e2, e6), (e3, e7) of 16-bit floats, exactly.  A nibble n is
-// the code q = (n ^ 8) - 8.  n ^ 8 put into the last mantissa bits of a power of two whose last place is 1 (bf16 128, fp16 1024)
-// reads as that power plus q + 8, so one subtraction leaves q; fp16 has room to take a nibble four bits up (its last place then
-// counts 1/16) and saves shifts.
+// Eight codes e0 .. e7 of one word -> four pairs (e0, e4), (e1, e5), (e2, e6), (e3, e7) of 16-bit floats, exactly: q for fp16, q / 4
+// for bf16 (kCodeUnit).  A nibble n is the code q = (n ^ 8) - 8; u = n ^ 8 is made to read as a float and one fma takes the 8 away.
+//   In the last mantissa bits of a power of two whose last place is 1 (bf16 128, fp16 1024) u reads as that power plus u.
+//   fp16 has room for a nibble four bits up, whose last place then counts 1/16.
+//   bf16 has not, but there bits 4 .. 7 with nothing above them are a (sub)normal number u 2^-129: the lowest exponent bit goes
+//   on where the mantissa ends.  fma.bf16x2 keeps subnormal numbers, and 2^127 is the largest factor, hence the quarter.
+// So one shift serves four pairs instead of three.
+template <typename T>
+constexpr float kCodeUnit = 1.0f;
+template <>
+constexpr float kCodeUnit<__nv_bfloat16> = 4.0f;
+
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
 {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = fma2(and_xor(w >> (4 * i), 0x000F000Fu, 0x43084308u), 0x3F803F80u, 0xC308C308u, tag);  // x 1 - 136
+    const uint32_t w8 = w >> 8;
+    c[0] = fma2(and_xor(w, 0x000F000Fu, 0x43084308u), 0x3E803E80u, 0xC208C208u, tag);   // x 1/4 - 34
+    c[1] = fma2(and_xor(w, 0x00F000F0u, 0x00800080u), 0x7F007F00u, 0xC000C000u, tag);   // x 2^127 - 2
+    c[2] = fma2(and_xor(w8, 0x000F000Fu, 0x43084308u), 0x3E803E80u, 0xC208C208u, tag);
+    c[3] = fma2(and_xor(w8, 0x00F000F0u, 0x00800080u), 0x7F007F00u, 0xC000C000u, tag);
 }
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__half> tag)
 {
@@ -157,14 +168,12 @@ __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag
     c[3] = fma2(and_xor(w8, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u, tag);
 }
 
-// The same eight codes in their own order: (e0, e1), (e2, e3), (e4, e5), (e6, e7).  A byte permute puts a byte's two nibbles into
-// the two halves: bf16 takes the high one from a copy of the word shifted by four, fp16 takes it where it is (see above).
+// The same eight codes (in the same unit) in their own order: (e0, e1), (e2, e3), (e4, e5), (e6, e7).  A byte permute puts a byte
+// into both halves of a word; one half keeps the low nibble, the other the high one.
 __device__ __forceinline__ void codes_in_order(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
 {
-    const uint32_t w4 = w >> 4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        c[j] = fma2(and_xor(__byte_perm(w, w4, 0x4400 + 0x1111 * j), 0x000F000Fu, 0x43084308u), 0x3F803F80u, 0xC308C308u, tag);
+    for (int j = 0; j < 4; ++j) c[j] = fma2(and_xor(__byte_perm(w, 0u, 0x1111 * j), 0x00F0000Fu, 0x00804308u), 0x7F003E80u, 0xC000C208u, tag);
 }
 __device__ __forceinline__ void codes_in_order(uint32_t w, uint32_t (&c)[4], Tag<__half> tag)
 {

@@ -4,7 +4,7 @@
 // Bound by memory: every element is read once and leaves as half a byte.  A lane takes eight consecutive elements (one or two
 // 16-byte loads) and writes their four bytes; 4, 8, 16 or 32 neighbouring lanes share a group, whose maximum is a few shuffles.
 // A warp has kUnroll such pieces of 256 elements in flight.
-#include <cstdlib>
+#include <type_traits>
 
 #include "qm_ptx.cuh"
 #include "qm_w4.cuh"
@@ -66,8 +66,48 @@ struct Eight {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
     }
-    __device__ __forceinline__ float at(int i) const { return to_float(reinterpret_cast<const T *>(v)[i]); }
+    __device__ __forceinline__ float at(int i) const
+    {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(v)[i >> 1];
+            return __uint_as_float((i & 1) ? w & 0xFFFF0000u : w << 16);
+        } else {
+            return to_float(reinterpret_cast<const T *>(v)[i]);
+        }
+    }
+    // The largest magnitude as the bits of T (two of them for 16-bit types, in both halves of the word): magnitudes order like
+    // unsigned integers, and an infinity or a NaN is above every number.
+    __device__ __forceinline__ uint32_t magnitude() const
+    {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) {
+            if constexpr (sizeof(T) == 4) m = max(m, w[i] & 0x7FFFFFFFu);
+            else m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        }
+        return m;
+    }
 };
+
+template <typename T>
+__device__ __forceinline__ uint32_t larger_magnitude(uint32_t a, uint32_t b)
+{
+    if constexpr (sizeof(T) == 4) return max(a, b);
+    else return __vmaxu2(a, b);
+}
+
+template <typename T>
+__device__ __forceinline__ float magnitude_value(uint32_t m)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(m);
+    } else {
+        const unsigned short h = (unsigned short)max(m & 0xFFFFu, m >> 16);
+        if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
+        else return __uint_as_float((uint32_t)h << 16);
+    }
+}
 
 // k % 8 == 0 and rows on 16-byte boundaries.  Pieces of 256 elements are dealt to the warps.
 template <typename T, typename S>
@@ -95,23 +135,37 @@ __global__ void __launch_bounds__(kThreads) quantize_w4_kernel(const T *__restri
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float a = 0.0f, bad = 0.0f;  // bad becomes NaN with any NaN: max drops them
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = w[u].at(j);
-                a = fmaxf(a, fabsf(v));
-                bad = v != v ? v : bad;
-            }
-            unsigned nan = __ballot_sync(0xFFFFFFFFu, bad != bad);
-            for (int d = 1; d < lanes; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, d));
-            nan &= (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (lane & ~(lanes - 1));
-            if (nan) a = __int_as_float(0x7FC00000);
-            const S stored = from_float<S>(__fmul_rn(a, 1.0f / 7.0f));
+            uint32_t m = w[u].magnitude();
+            for (int d = 1; d < lanes; d <<= 1) m = larger_magnitude<T>(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+            const S stored = from_float<S>(__fmul_rn(magnitude_value<T>(m), 1.0f / 7.0f));
             const Quotient z = quotient_for(stored);
             uint32_t word = 0;
-            if (z.some) {
+            // t = w / s to within two of its last places (|t| is at most 7.1 unless the scale lost digits, as a subnormal fp16 does),
+            // rounded by adding and taking away 1.5 x 2^23; that is the quotient's rounding unless t is next to a middle
+            float r[8], edge = 0.0f;
+            constexpr float kRound = 12582912.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) word |= (uint32_t)(code_of(w[u].at(j), z) & 15) << (4 * j);
+            for (int j = 0; j < 8; ++j) {
+                const float q = w[u].at(j) * z.inv;
+                r[j] = __fadd_rn(__fadd_rn(q, kRound), -kRound);
+                edge = fmaxf(edge, fabsf(q - r[j]));
+            }
+            // codes + 8 as base-16 digits, four in one fp32 whole number; the digits' high bits are then turned round
+            const float low = fmaf(r[3], 4096.0f, fmaf(r[2], 256.0f, fmaf(r[1], 16.0f, r[0]))) + (8388608.0f + 34952.0f);
+            const float high = fmaf(r[7], 4096.0f, fmaf(r[6], 256.0f, fmaf(r[5], 16.0f, r[4]))) + (8388608.0f + 34952.0f);
+            word = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410) ^ 0x88888888u;
+            if (!z.some) {
+                word = 0;
+            } else if (!(edge < 0.4999f) || z.up != 1.0f || (sizeof(S) == 2 && std::is_same<S, __half>::value && z.s < 0x1p-14f)) {
+                word = 0;
+#pragma unroll 1
+                for (int j = 0; j < 8; ++j) {
+                    // (not unrolled: rare, and eight copies would cost the common path its registers)
+                    float v = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v = i == j ? w[u].at(i) : v;
+                    word |= (uint32_t)(code_of(v, z) & 15) << (4 * j);
+                }
             }
             if (at[u] < k) {
                 __stcs(reinterpret_cast<uint32_t *>(packed + row[u] * (k / 2) + at[u] / 2), word);

@@ -6,7 +6,8 @@
 //
 //   warp 0       TMA producer of B: packed rows (64-byte swizzle) into a ring of kRingW stages of 8 KB
 //   warp 2       TMA producer of X: two 64-element sub-blocks (128-byte swizzle) of up to 128 rows into a ring of kRingX stages
-//   warps 12-19  converters, two sets of four that take the stages in turn; a thread owns a row of B: 64 bytes of codes become 128
+//   warp 3       relay of X's arrival to the MMA issuer
+//   warps 12-    converters, kSets sets of four that take the stages in turn; a thread owns a row of B: 64 bytes of codes become 128
 //                scaled 16-bit values in 64 TMEM columns (tcgen05.st)
 //   warp 1       MMA issuer (of the pair's leader): eight tcgen05.mma.kind::f16 a stage, fp32 accumulators in 256 TMEM columns
 //   warps 4-11   epilogue: two warps per lane quarter; lanes hold consecutive columns of out
@@ -18,7 +19,7 @@
 //
 // PAIR form (G = 2, persistent): two CTAs share a 256 x N tile, N <= 256; each converts its own 128 rows of B and loads half
 // of the rows of X, so a stage brings 24 KB into each SM for 1024 tensor clocks (a 128-row tile would need twice X's part).
-// N follows the rows that are left, in steps of 32: with experts a short segment costs its own width.
+// N follows the rows that are left, in steps of 16: with experts a short segment costs its own width.
 // SPLIT form (G = 1): where there are few tiles, a cluster of up to 8 CTAs shares one 128 x N tile, N <= 128, each taking a
 // part of K; the partial tiles meet in the CTAs' shared memory and are added in a fixed order.
 // All waits are bounded as in gemm_tc_kernel.
@@ -42,20 +43,20 @@ using namespace tc;
 
 constexpr int kRowsB = 128;     // rows of B per CTA
 constexpr int kStageK = 128;    // elements of K per stage
-constexpr int kRingW = 8, kRingX = 4;
+constexpr int kRingW = 7, kRingX = 4;
 constexpr int kBytesW = kRowsB * kStageK / 2;  // 8 KB
 constexpr int kRowsX = 128;                    // rows of X a CTA holds
 constexpr int kSubX = kRowsX * 128;            // 64 elements of K: 16 KB
 constexpr int kBytesX = 2 * kSubX;
 constexpr int kBoxRows = 32;
 constexpr int kAccCols = 256, kStageCols = 64, kTmemCols = 512;
-constexpr int kEpiWarp = 4, kNumEpiWarps = 8, kConvWarp = 12, kNumConvWarps = 8;
+constexpr int kEpiWarp = 4, kNumEpiWarps = 8, kConvWarp = 12, kSets = 3, kNumConvWarps = 4 * kSets;
 constexpr int kNumWarps = kConvWarp + kNumConvWarps, kNumThreads = kNumWarps * 32;
 constexpr int kNumBarriers = 2 * kRingW + 3 * kRingX + 2;
-constexpr int kSmemFixed = 1024 + kRingW * kBytesW + kRingX * kBytesX + kNumBarriers * 8 + 16 + kRowsB * 4;
+constexpr int kEpiBytes = 16 * 32 * 2;  // per epilogue warp: 16 rows of out x 32 columns
+constexpr int kSmemFixed = 1024 + kRingW * kBytesW + kRingX * kBytesX + kNumEpiWarps * kEpiBytes + kNumBarriers * 8 + 16 + kRowsB * 4;
 static_assert(kAccCols + kRingX * kStageCols <= kTmemCols, "TMEM budget");
 static_assert(kSmemFixed + 8 * 4097 <= 232448, "shared memory");
-static_assert(kRingX % 2 == 0, "the converter sets take stages in turn");
 
 struct TcParams {
     const void *scales;
@@ -64,11 +65,27 @@ struct TcParams {
     int64_t ldo;
     int rows, n, k, experts;
     int group_shift, groups;
-    int tile;        // rows of X per tile: a multiple of 16 (32 in the PAIR form)
+    int tile;        // rows of X per tile: a multiple of 16
     int vec_scales;  // the four scales of a stage (groups of 32), or two (64), can be loaded as one vector
-    int vec_out;     // out's rows begin on 4-byte boundaries
+    int vec_out;     // out's rows begin on 16-byte boundaries
     int *status;
 };
+
+// One lane of the (converged) warp, always the same one.  The code around it stays uniform over the warp, so that the compiler
+// keeps descriptors and addresses in uniform registers, which is where tcgen05.mma takes them: issued from a divergent branch
+// an MMA cost 85 clocks, most of them moves.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        " .reg .pred p;\n"
+        " elect.sync _|p, 0xFFFFFFFF;\n"
+        " selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(r));
+    return r != 0;
+}
 
 // D[tmem] (+)= A[tmem] * B[smem desc], 16-bit floats -> fp32.  One thread issues it.
 template <int G>
@@ -177,13 +194,15 @@ __device__ __forceinline__ float row_unit(const S *__restrict__ s, int groups)
 
 template <int G, typename T, typename S>
 __global__ void __launch_bounds__(kNumThreads, 1)
-w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ CUtensorMap tmapX, const TcParams p)
+w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ CUtensorMap tmapX, const __grid_constant__ CUtensorMap tmapX128,
+             const TcParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_u32 = smem_u32(smem_raw);
     const uint32_t x0 = (raw_u32 + 1023u) & ~1023u;   // X ring: [stage][sub-block][row][128 B]
     const uint32_t w0 = x0 + kRingX * kBytesX;        // B ring: [stage][row][64 B]
-    const uint32_t bar0 = w0 + kRingW * kBytesW;
+    const uint32_t epi0 = w0 + kRingW * kBytesW;      // epilogue: [warp][row of X][32 columns]
+    const uint32_t bar0 = epi0 + kNumEpiWarps * kEpiBytes;
     auto w_full = [&](int s) { return bar0 + 8u * s; };
     auto w_empty = [&](int s) { return bar0 + 8u * (kRingW + s); };
     auto x_full = [&](int s) { return bar0 + 8u * (2 * kRingW + s); };
@@ -209,7 +228,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRingW; ++s) mbar_init(w_full(s), 1), mbar_init(w_empty(s), 4);
-        for (int s = 0; s < kRingX; ++s) mbar_init(x_full(s), 1), mbar_init(a_full(s), 4 * G), mbar_init(ax_empty(s), 1);
+        for (int s = 0; s < kRingX; ++s) mbar_init(x_full(s), 1), mbar_init(a_full(s), 5 * G), mbar_init(ax_empty(s), 1);
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, G * kNumEpiWarps);
         *abort_flag = 0;
@@ -217,7 +236,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
         fence_proxy_async_smem();
     }
     if (warp == 0 && lane == 0) prefetch_tmap(&tmapW);
-    if (warp == 2 && lane == 0) prefetch_tmap(&tmapX);
+    if (warp == 2 && lane == 0) prefetch_tmap(&tmapX), prefetch_tmap(&tmapX128);
     if (warp == 1) {
         tmem_alloc<G>(tmem_slot, kTmemCols);
         tmem_relinquish<G>();
@@ -251,7 +270,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
         tile_coords(local, tilesP, (last - first + p.tile - 1) / p.tile, tp, tq);
         it.row = first + tq * p.tile;
         it.count = min(p.tile, last - it.row);
-        it.width = (it.count + 16 * G - 1) & ~(16 * G - 1);
+        it.width = (it.count + 15) & ~15;
         it.col = tp * kRowsB * G;
         return it;
     };
@@ -262,84 +281,119 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
 
     if (warp == 0) {
         // ------------------------------ producer of B ------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = cluster; t < num_items && ok; t += clusters) {
-                const Item m = item(t);
-                const int y = m.e * p.n + m.col + (G == 2 ? rank * kRowsB : 0);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % kRingW;
-                    if (!mbar_wait(w_empty(s), ((it / kRingW) & 1u) ^ 1u, abort_flag)) {
-                        give_up(kWaitProducerSlot);
-                        ok = false;
-                        break;
-                    }
+        const bool elected = elect_one();
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = cluster; t < num_items && ok; t += clusters) {
+            const Item m = item(t);
+            const int y = m.e * p.n + m.col + (G == 2 ? rank * kRowsB : 0);
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % kRingW;
+                if (!warp_wait<false>(w_empty(s), ((it / kRingW) & 1u) ^ 1u, abort_flag, lane)) {
+                    if (lane == 0) give_up(kWaitProducerSlot);
+                    ok = false;
+                    break;
+                }
+                if (elected) {
                     mbar_arrive_expect_tx(w_full(s), kBytesW);
                     tma_load_2d(w0 + s * kBytesW, &tmapW, kb * (kStageK / 2), y, w_full(s));
                 }
+                __syncwarp();
             }
         }
-        __syncwarp();
     } else if (warp == 2) {
         // ------------------------------ producer of X ------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = cluster; t < num_items && ok; t += clusters) {
-                const Item m = item(t);
-                const int share = m.width / G, boxes = (share + kBoxRows - 1) / kBoxRows;
-                const int y = m.row + (G == 2 ? rank * share : 0);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % kRingX;
-                    if (!mbar_wait(ax_empty(s), ((it / kRingX) & 1u) ^ 1u, abort_flag)) {
-                        give_up(kWaitProducerSlot);
-                        ok = false;
-                        break;
-                    }
-                    mbar_arrive_expect_tx(x_full(s), (uint32_t)boxes * 2 * kBoxRows * 128);
-                    for (int h = 0; h < 2; ++h)
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(x0 + s * kBytesX + h * kSubX + b * kBoxRows * 128, &tmapX, kb * kStageK + h * 64, y + b * kBoxRows, x_full(s));
+        const bool elected = elect_one();
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = cluster; t < num_items && ok; t += clusters) {
+            const Item m = item(t);
+            const int share = m.width / G, boxes = (share + kBoxRows - 1) / kBoxRows;
+            const bool whole = boxes == kRowsX / kBoxRows;  // one box per sub-block
+            const int y = m.row + (G == 2 ? rank * share : 0);
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % kRingX;
+                if (!warp_wait<false>(ax_empty(s), ((it / kRingX) & 1u) ^ 1u, abort_flag, lane)) {
+                    if (lane == 0) give_up(kWaitProducerSlot);
+                    ok = false;
+                    break;
                 }
+                if (elected) {
+                    const uint32_t dst = x0 + s * kBytesX;
+                    mbar_arrive_expect_tx(x_full(s), (uint32_t)boxes * 2 * kBoxRows * 128);
+                    if (whole) {
+                        tma_load_2d(dst, &tmapX128, kb * kStageK, y, x_full(s));
+                        tma_load_2d(dst + kSubX, &tmapX128, kb * kStageK + 64, y, x_full(s));
+                    } else {
+                        for (int b = 0; b < boxes; ++b) {
+                            tma_load_2d(dst + b * kBoxRows * 128, &tmapX, kb * kStageK, y + b * kBoxRows, x_full(s));
+                            tma_load_2d(dst + kSubX + b * kBoxRows * 128, &tmapX, kb * kStageK + 64, y + b * kBoxRows, x_full(s));
+                        }
+                    }
+                }
+                __syncwarp();
             }
         }
-        __syncwarp();
+    } else if (warp == 3) {
+        // ------------------------------ relay: this CTA's rows of X have arrived ------------------------------
+        // The MMA issuer waits for one signal per stage that covers both operands of both CTAs.
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = cluster; t < num_items && ok; t += clusters) {
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % kRingX;
+                if (!warp_wait<false>(x_full(s), (it / kRingX) & 1u, abort_flag, lane)) {
+                    if (lane == 0) give_up(kWaitMmaOperands);
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    if constexpr (G == 2) mbar_arrive_cluster(a_full(s), 0);
+                    else mbar_arrive(a_full(s));
+                }
+                __syncwarp();
+            }
+        }
     } else if (warp == 1) {
         // ------------------------------ MMA issuer ------------------------------
-        if (lane == 0 && (G == 1 || rank == 0)) {
+        if (G == 1 || rank == 0) {  // uniform over the warp, as is everything below but the elected lane
             constexpr uint32_t kFormat = std::is_same<T, __half>::value ? 0u : 1u;  // of both operands
+            const bool elected = elect_one();
             uint32_t it = 0, lt = 0;
             bool ok = true;
             for (int t = cluster; t < num_items && ok; t += clusters, ++lt) {
                 const Item m = item(t);
                 const uint32_t idesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(m.width >> 3) << 17) | ((uint32_t)(128 * G >> 4) << 24);
-                if (!mbar_wait(acc_empty, (lt & 1u) ^ 1u, abort_flag)) {
-                    give_up(kWaitMmaAcc);
+                if (!warp_wait<false>(acc_empty, (lt & 1u) ^ 1u, abort_flag, lane)) {
+                    if (lane == 0) give_up(kWaitMmaAcc);
                     break;
                 }
                 tc_fence_after_sync();
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = it % kRingX;
-                    if (!mbar_wait(a_full(s), (it / kRingX) & 1u, abort_flag)) {
-                        give_up(kWaitMmaOperands);
+                    if (!warp_wait<false>(a_full(s), (it / kRingX) & 1u, abort_flag, lane)) {
+                        if (lane == 0) give_up(kWaitMmaOperands);
                         ok = false;
                         break;
                     }
                     tc_fence_after_sync();
+                    const uint64_t dX = make_smem_desc(x0 + s * kBytesX);
+                    const uint32_t ta = tmem_a0 + (uint32_t)(s * kStageCols);
+                    if (elected) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint64_t dX = make_smem_desc(x0 + s * kBytesX + h * kSubX);
-                        const uint32_t ta = tmem_a0 + (uint32_t)(s * kStageCols + h * 32);
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int k4 = 0; k4 < 4; ++k4) umma_f16_ta<G>(tmem_base, ta + 8u * k4, dX + 2u * k4, idesc, (kb != kb0 || (h | k4) != 0) ? 1u : 0u);
+                            for (int k4 = 0; k4 < 4; ++k4)
+                                umma_f16_ta<G>(tmem_base, ta + 32u * h + 8u * k4, dX + (uint64_t)(h * (kSubX >> 4) + 2 * k4), idesc,
+                                               (h | k4) != 0 ? 1u : (kb != kb0 ? 1u : 0u));
+                        commit_all<G>(ax_empty(s));
                     }
-                    commit_all<G>(ax_empty(s));
+                    __syncwarp();
                 }
-                if (ok) commit_all<G>(acc_full);
+                if (ok && elected) commit_all<G>(acc_full);
+                __syncwarp();
             }
         }
-        __syncwarp();
     } else if (warp >= kConvWarp) {
         // ------------------------------ converters ------------------------------
         const int set = (warp - kConvWarp) >> 2, quarter = warp & 3;
@@ -389,17 +443,17 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                     }
                 }
             };
-            // this set's stages of the item are those with (it + kb - kb0) % 2 == set
-            const int first_kb = kb0 + (((it & 1u) == (uint32_t)set) ? 0 : 1);
+            // this set's stages of the item are those with (it + kb - kb0) % kSets == set
+            const int first_kb = kb0 + (int)(((uint32_t)(set + kSets) - it % kSets) % kSets);
             float next[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (live && first_kb < kb1) load_scales(first_kb, next);
-            for (int kb = first_kb; kb < kb1; kb += 2) {
+            for (int kb = first_kb; kb < kb1; kb += kSets) {
                 const uint32_t i = it + (uint32_t)(kb - kb0);
                 const int ws = i % kRingW, s = i % kRingX;
                 float sc[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sc[j] = next[j] * inv;
-                if (live && kb + 2 < kb1) load_scales(kb + 2, next);
+                for (int j = 0; j < 4; ++j) sc[j] = next[j] * (inv * kCodeUnit<T>);
+                if (live && kb + kSets < kb1) load_scales(kb + kSets, next);
                 if (!warp_wait<false>(w_full(ws), (i / kRingW) & 1u, abort_flag, lane)) {
                     if (lane == 0) give_up(kWaitConvertPacked);
                     ok = false;
@@ -446,12 +500,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                 }
                 tmem_st_wait();
                 tc_fence_before_sync();
-                // this CTA's rows of X are there too: one signal covers both operands
-                if (!warp_wait<false>(x_full(s), (i / kRingX) & 1u, abort_flag, lane)) {
-                    if (lane == 0) give_up(kWaitConvertPacked);
-                    ok = false;
-                    break;
-                }
                 __syncwarp();
                 if (lane == 0) {
                     if constexpr (G == 2) mbar_arrive_cluster(a_full(s), 0);
@@ -466,7 +514,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
         const int r = quarter * 32 + lane;
         const S *__restrict__ scales = static_cast<const S *>(p.scales);
         T *__restrict__ out = static_cast<T *>(p.out);
-        const bool odd = (lane & 1) != 0;
         uint32_t lt = 0;
         for (int t = cluster; t < num_items; t += clusters, ++lt) {
             const Item m = item(t);
@@ -481,6 +528,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
             }
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+            const uint32_t buf = epi0 + (uint32_t)((warp - kEpiWarp) * kEpiBytes);
+            const int col0 = c - lane;  // the warp's first column
             const int chunks = m.width / 16;
             for (int ch = half; ch < chunks; ch += 2) {
                 uint32_t v[16];
@@ -499,25 +548,35 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                     for (int j = 0; j < 16; ++j) part[(ch * 16 + j) * kRowsB + r] = __uint_as_float(v[j]);
                     continue;
                 }
+                // through the warp's buffer, so that a store writes 64 contiguous bytes of eight rows.  (Straight from the
+                // registers, two bytes a lane and one row at a time behind bounds checks, the epilogue took 11,800 clocks of a
+                // tile whose MMAs take 32,700.)
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
-                    // two rows of out: even lanes take columns (c, c + 1) of the first, odd lanes (c - 1, c) of the second
-                    const float a = __uint_as_float(v[j]) * unit, b = __uint_as_float(v[j + 1]) * unit;
-                    const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 1);
-                    const uint32_t two = odd ? pack2(got, b, Tag<T>()) : pack2(a, got, Tag<T>());
-                    const int row = ch * 16 + j + (odd ? 1 : 0);
-                    const int col = c & ~1;
-                    if (row < m.count) {
-                        T *dst = out + (int64_t)(m.row + row) * p.ldo + col;
-                        if (p.vec_out && col + 1 < p.n) {
-                            *reinterpret_cast<uint32_t *>(dst) = two;
-                        } else {
-                            unsigned short *d16 = reinterpret_cast<unsigned short *>(dst);
-                            if (col < p.n) d16[0] = (unsigned short)two;
-                            if (col + 1 < p.n) d16[1] = (unsigned short)(two >> 16);
-                        }
+                    const uint32_t two = pack2(__uint_as_float(v[j]) * unit, __uint_as_float(v[j + 1]) * unit, Tag<T>());
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(buf + j * 64 + lane * 2), "h"((unsigned short)two) : "memory");
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(buf + j * 64 + 64 + lane * 2), "h"((unsigned short)(two >> 16)) : "memory");
+                }
+                __syncwarp();
+                const int row0 = ch * 16, sub = lane >> 2, piece = (lane & 3) * 8;
+                T *dst = out + (int64_t)(m.row + row0 + sub) * p.ldo + col0 + piece;
+                const uint4 a0 = lds128(buf + lane * 16), a1 = lds128(buf + 512 + lane * 16);
+                if (p.vec_out && row0 + 16 <= m.count && col0 + 32 <= p.n) {
+                    *reinterpret_cast<uint4 *>(dst) = a0;
+                    *reinterpret_cast<uint4 *>(dst + 8 * p.ldo) = a1;
+                } else {
+#pragma unroll 1
+                    for (int o = 0; o < 2; ++o, dst += 8 * p.ldo) {
+                        if (row0 + sub + 8 * o >= m.count) continue;
+                        const uint4 a = o ? a1 : a0;
+                        const uint32_t word[4] = {a.x, a.y, a.z, a.w};
+                        unsigned short *d16 = reinterpret_cast<unsigned short *>(dst);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (col0 + piece + j < p.n) d16[j] = (unsigned short)(word[j >> 1] >> (16 * (j & 1)));
                     }
                 }
+                __syncwarp();  // the buffer is rewritten next
             }
             // a warp whose half has no columns hands the accumulator back as well
             if (G == 2 && half >= chunks) {
@@ -573,13 +632,13 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
     }
 }
 
-int make_x_tmap(CUtensorMap *map, const W4Args &a)
+int make_x_tmap(CUtensorMap *map, const W4Args &a, int box_rows)
 {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return record_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled entry point");
     cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
     cuuint64_t strides[1] = {(cuuint64_t)a.ldx * 2};
-    cuuint32_t box[2] = {64, kBoxRows};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(map, a.type == QM_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(a.X), dims,
                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -635,9 +694,10 @@ int tc_launch_variant(const W4Args &a, const TcPlanW4 &plan, const DeviceCtx &ct
 {
     auto kernel = w4_tc_kernel<G, T, S>;
     const size_t smem = kSmemFixed + (size_t)(a.experts + 1) * 8;
-    CUtensorMap tmW, tmX;
+    CUtensorMap tmW, tmX, tmX128;
     int st = make_packed_tmap(&tmW, a.B, a.experts * a.n, a.k / 2, kRowsB, CU_TENSOR_MAP_SWIZZLE_64B);
-    if (st == QM_OK) st = make_x_tmap(&tmX, a);
+    if (st == QM_OK) st = make_x_tmap(&tmX, a, kBoxRows);
+    if (st == QM_OK) st = make_x_tmap(&tmX128, a, kRowsX);
     if (st != QM_OK) return st;
     TcParams p;
     p.scales = a.scales, p.offsets = a.offsets, p.out = a.out, p.ldo = a.ldo;
@@ -647,7 +707,7 @@ int tc_launch_variant(const W4Args &a, const TcPlanW4 &plan, const DeviceCtx &ct
     p.tile = plan.tile;
     const int gps = a.group >= 128 ? 1 : 128 / a.group;
     p.vec_scales = p.groups % gps == 0 && (reinterpret_cast<uintptr_t>(a.scales) & (gps * sizeof(S) - 1)) == 0;
-    p.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0 && (a.ldo & 1) == 0;
+    p.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && (a.ldo & 7) == 0;
     p.status = ctx.status;
 
     const int64_t tilesP = (a.n + kRowsB * G - 1) / (kRowsB * G);
@@ -674,7 +734,7 @@ int tc_launch_variant(const W4Args &a, const TcPlanW4 &plan, const DeviceCtx &ct
     cfg.attrs = attr;
     static const bool allow_pdl = !std::getenv("QM_NO_PDL");
     cfg.numAttrs = allow_pdl ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, tmX128, p);
     return e == cudaSuccess ? QM_OK : record_cuda_error(e, "w4_tc_kernel launch");
 }
 
@@ -683,6 +743,7 @@ TcPlanW4 tc_plan(const W4Args &a, const DeviceCtx &ctx)
 {
     TcPlanW4 plan = {1, 256, 1};
     const int num_kb = (a.k + kStageK - 1) / kStageK;
+    const int pairs = ctx.num_sms / 2;
     if (a.offsets) {
         // a tile holds an average segment
         const int average = a.rows / (a.experts < a.rows ? a.experts : a.rows);
@@ -698,6 +759,17 @@ TcPlanW4 tc_plan(const W4Args &a, const DeviceCtx &ctx)
         if (parts > 8) parts = 8;
         if (parts > num_kb) parts = num_kb;
         plan.parts = parts < 1 ? 1 : parts;
+        return plan;
+    }
+    // PAIR form: tiles go round over the pairs, and a tile costs its width plus the epilogue and the refill of the pipeline, which
+    // take about as long as 12 columns of an average main loop.  The width with the fewest rounds' cost: 2048 x 12288 has 384 tiles
+    // of 256 rows, six rounds of 74 pairs, but 432 of 240, six rounds of 0.94 of the length.  (Below 192 the converters and
+    // the loads of B no longer hide behind the MMAs.)
+    double best = 0.0;
+    for (int width = 256; width >= 192; width -= 16) {
+        const int64_t tiles = (int64_t)((a.n + 255) / 256) * ((a.rows + width - 1) / width);
+        const double cost = (double)((tiles + pairs - 1) / pairs) * (width + 12);
+        if (best == 0.0 || cost < best) best = cost, plan.tile = width;
     }
     return plan;
 }
