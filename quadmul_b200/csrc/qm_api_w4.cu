@@ -33,7 +33,7 @@ int w4_dispatch(const W4Args &a)
     st = device_ctx(&ctx);
     if (st != QM_OK) return st;
     const int average = a.rows / (a.experts < a.rows ? a.experts : a.rows);
-    if (average <= (a.offsets ? 8 : 16) && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
+    if (average <= 8 && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
     if (w4_tc_eligible(a)) return w4_tc_launch(a, *ctx);
     return w4_simt_launch(a);
 }

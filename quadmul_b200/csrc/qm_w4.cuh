@@ -76,6 +76,22 @@ inline int launched(const char *what)
     return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
 }
 
+// One lane of the (converged) warp, always the same one.  The code around it stays uniform over the warp, so that the compiler
+// keeps descriptors and addresses in uniform registers, which is where tcgen05.mma and TMA instructions take them: issued from a
+// divergent branch an MMA cost 85 clocks, most of them moves, and 28 from uniform code.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        " .reg .pred p;\n"
+        " elect.sync _|p, 0xFFFFFFFF;\n"
+        " selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(r));
+    return r != 0;
+}
+
 // The experts' segments, from offsets that may be anything: seg[e] (e = 0 .. experts) is the running maximum of the offsets
 // clamped to [0, rows], so expert e has the rows [seg[e], seg[e + 1]); tiles[e] is how many tiles of `tile` rows the experts
 // below e have.  Run by one warp; seg and tiles are shared memory, to be read after a barrier.

@@ -1,20 +1,30 @@
 // 4-bit weights with group scales, few rows of X: weight streaming.
 //
-// out[r][c] = sum over groups g of scale[c][g] * sum over i in g of x[r][i] q[c][i].  With up to 16 rows of X the product reads
-// every weight once and is bound by memory; what a kernel has to do is keep loads in flight and convert codes fast enough.
+// out[r][c] = sum over groups g of scale[c][g] * sum over i in g of x[r][i] q[c][i].  With a few rows of X the product reads every
+// weight once and should be bound by memory; what costs is making operands of the codes.  As 16-bit floats they take nine
+// instructions per eight codes, and a kernel built that way stood at half of the HBM rate with its issue slots full.  As int8 (times
+// 16, nibble in the high half of the byte) they take three.  So X becomes whole numbers instead, once per launch and CTA:
 //
-//  * A CTA (16 warps) takes blocks of 8 RG rows of B, WK of its warps split K between them in steps of 128 elements.  Every
-//    warp has a ring of p.depth boxes (8 RG rows x 64 bytes) of its own, filled by TMA loads that its first lane issues as soon
-//    as a box has been read: no other warp takes part, the loads run on across the end of a block, and up to 128 KB are on the
-//    way per SM.  Lane (g, q) = (lane / 4, lane % 4) reads 16 bytes, 32 codes, of row g of each 8-row group.
-//  * The product runs on mma.sync.m16n8k16: 16 rows of B x 8 rows of X.  The codes become 16-bit floats in registers, exactly
-//    (codes_to_pairs), and the sums of a group are exact products added in fp32; the group's scale is applied to the fp32 sum, so
-//    no weight is ever rounded.  The order of K inside an instruction is free as long as both operands use the same one: a word of
-//    eight codes unpacks into pairs (e0, e4) .. (e3, e7), and the rows of X are put into that order once, when they are staged.
-//  * One instruction adds up over the four lanes of a row, so these must hold codes of one group: with groups of 128 and more
-//    every lane uses its own 32 codes; for groups of 64 and 32 the lanes of a row trade words (4 or 8 shuffles a step).
-//  * The rows of X that a warp needs (its share of K) sit in shared memory in the order of the lanes that read them: staged by
-//    the lane that uses them, so without a barrier, once for all blocks of an expert.
+//   In every stretch of K that shares a weight scale (at most 128 elements) the row of X is divided by a power of two above its
+//   largest value and rounded to 22 bits, v = d1 2^16 + d2 2^8 + d3 with signed bytes d.  The three dot products of a stretch
+//   are exact in int32 (mma.sync.m16n8k32), and scale * (d1 . q, d2 . q, d3 . q) is added in fp32, one rounding per stretch, as
+//   an fp32 sum of products would have one per product.  The only loss is that of elements below 2^-13 of their stretch's largest
+//   (bf16; 2^-10 for fp16): their last bits are rounded at 2^-22 of it, four times fp32's own last place.
+//   A row with an infinity or a NaN cannot be written so; its outputs are computed again, element by element.
+//
+//  * A CTA (16 warps) takes blocks of 32 rows of B per warp group; WK of its warps split K between them in steps of 128 elements.
+//    Lane (g, q) = (lane / 4, lane % 4) loads 16 bytes, 32 codes, of row g of each 8-row group straight into registers; kDepth steps
+//    are on the way per warp (64 KB per SM; a third costs registers that are not there), across the end of a block, so the
+//    stream does not stop there.  (TMA rings in their
+//    place, one per warp or one per CTA with a loading warp, were slower: a small box costs its thread about 400 clocks, and
+//    1 x 4096 x 4096 has time for four.)
+//  * A word's even and odd elements are the two halves of an operand fragment; which K an instruction's columns stand for is free
+//    as long as X is laid out alike.  But an instruction adds up over the four lanes of a row, so these must hold codes of
+//    one group: with groups of 128 and more every lane uses its own 32 codes; for 64 and 32 the lanes of a row trade words.
+//  * With many blocks of B fewer warps split K (WK) and there are more warp groups, which share the rows of X and nothing else: a
+//    group meets at a named barrier of its own at the end of its 32 rows, so that one adds up while another multiplies.
+//  * Rows of X sit in the eight columns of an instruction.  WIDE (3 to 8 rows): a column per row, an instruction per byte d.
+//    Otherwise (1 or 2 rows) the three bytes of both rows take six columns of one instruction.
 //  * The warps' partial tiles meet in shared memory (two buffers, one barrier a block) and are added in a fixed order.
 //
 // With experts a unit of work is (expert, tile of its rows, block of B); every CTA takes a contiguous range of units, so the rows
@@ -24,7 +34,6 @@
 #include <type_traits>
 
 #include "qm_ptx.cuh"
-#include "qm_tc_common.cuh"
 #include "qm_w4.cuh"
 
 namespace qm {
@@ -34,52 +43,45 @@ using namespace w4;
 namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32;
-constexpr int kMaxDepth = 4;     // boxes in flight per warp
-constexpr int kStep = 128;       // elements of K per step
+constexpr int kDepth = 2;                          // steps on the way per warp
+constexpr int kStep = 128;                         // elements of K per step
+constexpr int kRG = 4, kTiles = 2, kRows = 8 * kRG;  // 8-row groups, 16-row tiles and rows of B per warp
+constexpr int kRedFloats = kWarps * kTiles * 128;  // one of two buffers
 constexpr int kMaxSmem = 232448 - 1024;
+constexpr int kNarrowRows = 2, kWideRows = 8;
 
 struct RowsParams {
     const void *X;
     int64_t ldx;
+    const uint8_t *B;
     const void *scales;
     const int *offsets;
     void *out;
     int64_t ldo;
     int rows, n, k, experts;
     int group_shift, groups;
-    int tile;      // rows of X per unit, at most 16
-    int depth;     // boxes in a warp's ring
-    int *status;
-    int warps_k;   // warps that split K; the others take further rows of B
+    int warps_k;     // warps that split K; the others take further rows of B
     int vec_scales;  // a step's scales can be loaded as one vector
 };
 
-// d = a b, or d += a b: 16 rows of B x 16 elements of K x 8 rows of X
-template <typename T, bool FRESH>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+// d (+)= a b: 16 rows of B x 32 elements of K x 8 columns
+template <bool FRESH>
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    if constexpr (std::is_same<T, __half>::value) {
-        if constexpr (FRESH)
-            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-        else
-            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    } else {
-        if constexpr (FRESH)
-            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-        else
-            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    }
+    // a fresh sum starts at the bits of 1.5 x 2^23, so that what comes out reads as that number plus the sum (below 2^22)
+    if constexpr (FRESH)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0x4B400000));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// GPS scales of one step as they lie in memory
+__device__ __forceinline__ float sum_value(int d) { return __fadd_rn(__int_as_float(d), -12582912.0f); }
+
+// The GPS scales of one step as they lie in memory
 template <typename S, int GPS>
 struct RawScales {
     static constexpr int kWords = GPS * (int)sizeof(S) >= 4 ? GPS * (int)sizeof(S) / 4 : 1;
@@ -93,183 +95,264 @@ __device__ __forceinline__ float scale_at(const RawScales<S, GPS> &r, int j, int
         return __uint_as_float(__shfl_sync(0xFFFFFFFFu, r.w[j], src_lane));
     } else {
         const uint32_t v = __shfl_sync(0xFFFFFFFFu, r.w[j >> 1], src_lane);
-        const unsigned short h = (unsigned short)((j & 1) ? v >> 16 : v);
-        if constexpr (std::is_same<S, __half>::value) return __half2float(__ushort_as_half(h));
-        else return __bfloat162float(__ushort_as_bfloat16(h));
+        if constexpr (std::is_same<S, __half>::value) return __half2float(__ushort_as_half((unsigned short)((j & 1) ? v >> 16 : v)));
+        else return __uint_as_float((j & 1) ? v & 0xFFFF0000u : v << 16);
     }
 }
 
-// GPS = groups per step of 128 elements (4, 2 or 1 for groups of 32, 64, and 128 or more), RG = 8-row groups of B per warp,
-// TT = 8-row tiles of X.
-template <typename T, typename S, int GPS, int RG, int TT>
-__global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_constant__ CUtensorMap tmapB, const RowsParams p)
+// Barrier of `threads` threads; true for all of them if `any` is for one.
+__device__ __forceinline__ bool barrier_or(int id, int threads, bool any)
 {
-    constexpr int kTiles = RG / 2;            // 16-row tiles of B per warp
-    constexpr int kBoxBytes = 8 * RG * 64;
-    extern __shared__ __align__(128) uint4 smem_u4[];
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        " .reg .pred p, q;\n"
+        " setp.ne.u32 p, %3, 0;\n"
+        " barrier.cta.red.or.pred q, %1, %2, p;\n"
+        " selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(r)
+        : "r"(id), "r"(threads), "r"((uint32_t)any)
+        : "memory");
+    return r != 0;
+}
+
+// One output from its definition, in the order of K.
+template <typename T, typename S>
+__device__ __noinline__ float plain_output(const T *x, const uint8_t *b, const S *s, int k, int group)
+{
+    float sum = 0.0f;
+    for (int g0 = 0, g = 0; g0 < k; g0 += group, ++g) {
+        float part = 0.0f;
+        for (int i = g0; i < min(k, g0 + group); i += 2) {
+            const int byte = (int8_t)b[i >> 1];
+            part = fmaf(to_float(x[i]), (float)((int)((uint32_t)byte << 28) >> 28), part);
+            part = fmaf(to_float(x[i + 1]), (float)(byte >> 4), part);
+        }
+        sum = fmaf(to_float(s[g]), part, sum);
+    }
+    return sum;
+}
+
+// GPS = groups per step of 128 elements (4, 2 or 1 for groups of 32, 64, and 128 or more).
+template <typename T, typename S, int GPS, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p)
+{
+    constexpr int TT = WIDE ? 3 : 1;               // instructions per 16 rows of B and 32 elements of K
+    constexpr int kTile = WIDE ? kWideRows : kNarrowRows;  // rows of X per unit
+    constexpr int kColumns = 8;
+    constexpr int kPlace = 2 * TT * 32;            // 16-byte pieces of X per step
+    extern __shared__ uint4 smem_u4[];
     const T *__restrict__ X = static_cast<const T *>(p.X);
     const S *__restrict__ scales = static_cast<const S *>(p.scales);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int groups_of_rows = kWarps / p.warps_k;
     const int wk = warp % p.warps_k, wr = warp / p.warps_k;
-    const int block_rows = 8 * RG * (kWarps / p.warps_k);
+    const int block_rows = kRows * groups_of_rows;
     const int blocks = (p.n + block_rows - 1) / block_rows;
-    const int steps = (p.k + kStep - 1) / kStep;
-    const int slots = p.tile;                                     // staged rows of X
-    const int staged = (steps + p.warps_k - 1) / p.warps_k;       // steps a warp has room for
+    const int steps = (p.k + kStep - 1) / kStep, chunks = p.k / 32;
+    const uint32_t row_bytes = (uint32_t)p.k / 2;
+    // a warp has `mine` steps, WK apart (one without a step works on a place of zeros); X has a place for each, for all warp groups
     const int mine = max(1, (steps - wk + p.warps_k - 1) / p.warps_k);
+    const int places = max(steps, p.warps_k);
 
-    // ring [warp][box], X [warp][step][set][row][q] 16 bytes, partial tiles, barriers, segments
-    const uint32_t ring = ptx::smem_u32(smem_u4) + (uint32_t)(warp * p.depth * kBoxBytes);
-    uint4 *xs = smem_u4 + (kWarps * p.depth * kBoxBytes) / 16 + (size_t)warp * staged * 4 * slots * 4;
-    float *red = reinterpret_cast<float *>(smem_u4 + (kWarps * p.depth * kBoxBytes) / 16 + (size_t)kWarps * staged * 4 * slots * 4);
-    constexpr int kRedFloats = kWarps * kTiles * TT * 128;  // one of two buffers
-    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * kRedFloats);
-    const uint32_t bar0 = ptx::smem_u32(bars + warp * kMaxDepth);
-    int *abort_word = reinterpret_cast<int *>(bars + kWarps * kMaxDepth);
-    int *seg = abort_word + 2, *tiles = seg + p.experts + 1;
+    // X [place][pair of sets][instruction][lane] 16 bytes, X's units [place][group][column], partial tiles, rows of X that are not
+    // finite, segments
+    uint4 *xs = smem_u4;
+    float *unit = reinterpret_cast<float *>(smem_u4 + (size_t)places * kPlace);
+    float *red = unit + (size_t)places * GPS * kColumns;
+    unsigned *odd_rows = reinterpret_cast<unsigned *>(red + 2 * kRedFloats);  // [pair's parity][kWarps]
+    int *seg = reinterpret_cast<int *>(odd_rows + 2 * kWarps), *tiles = seg + p.experts + 1;
 
     ptx::grid_launch_dependents();
-    if (threadIdx.x == 0) *abort_word = 0;
-    if (lane == 0) {
-        for (int s = 0; s < p.depth; ++s) ptx::mbar_init(bar0 + 8u * s, 1);
-        ptx::fence_mbar_init();
-        ptx::fence_proxy_async_smem();
-        ptx::prefetch_tmap(&tmapB);
-        if (!p.offsets) {
-            // L2 prefetch of this warp's first boxes: returns no data, changes nothing the program can observe
-            const int row = (int)((int64_t)((p.rows + p.tile - 1) / p.tile) * blocks * blockIdx.x / gridDim.x) % blocks * block_rows + wr * 8 * RG;
-            for (int i = 0; i < min(mine, p.depth); ++i)
-                asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&tmapB), "r"((wk + i * p.warps_k) * 64), "r"(row) : "memory");
-        }
+    // CTA c takes the units from first_unit(c) up to first_unit(c + 1); the host has seen to it that their number fits an int
+    auto first_unit = [&](int units, unsigned c) {
+        const unsigned each = (unsigned)units / gridDim.x, more = (unsigned)units % gridDim.x;
+        return c * each + min(c, more);
+    };
+    const int row_tiles = (p.rows + kTile - 1) / kTile;
+    if (!p.offsets && (int)threadIdx.x < block_rows) {
+        // L2 prefetch of this CTA's first block: returns no data, changes nothing the program can observe
+        const int row = (int)(first_unit(row_tiles * blocks, blockIdx.x) % blocks) * block_rows + (int)threadIdx.x;
+        if (row < p.n) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.B + (int64_t)row * row_bytes), "r"(row_bytes) : "memory");
     }
     ptx::grid_dependency_wait();  // nothing above read or wrote global memory
 
-    int pairs;  // (expert, tile of rows)
+    int pairs = row_tiles;  // (expert, tile of rows)
     if (p.offsets) {
-        if (warp == 0) scan_segments(p.offsets, p.experts, p.rows, p.tile, seg, tiles, lane);
+        if (warp == 0) scan_segments(p.offsets, p.experts, p.rows, kTile, seg, tiles, lane);
         __syncthreads();
         pairs = tiles[p.experts];
-    } else {
-        __syncthreads();
-        pairs = (p.rows + p.tile - 1) / p.tile;
     }
-    const int64_t units = (int64_t)pairs * blocks;  // the host has seen to it that they fit an int
-    const int u_begin = (int)(units * blockIdx.x / gridDim.x), u_end = (int)(units * (blockIdx.x + 1) / gridDim.x);
+    const int u_begin = (int)first_unit(pairs * blocks, blockIdx.x), u_end = (int)first_unit(pairs * blocks, blockIdx.x + 1);
     if (u_begin >= u_end) return;
-
     auto expert_of = [&](int pair) { return p.offsets ? expert_of_tile(tiles, p.experts, pair) : 0; };
 
-    // ---- boxes of codes run p.depth steps ahead of the products
-    int lu = u_begin, li = 0, lslot = 0, lrow = 0;
-    auto load_box = [&]() {
-        if (lu >= u_end) return;
-        if (li == 0) {
-            const int pair = lu / blocks;
-            lrow = expert_of(pair) * p.n + (lu - pair * blocks) * block_rows + wr * 8 * RG;
-        }
-        if (lane == 0) {
-            ptx::mbar_arrive_expect_tx(bar0 + 8u * lslot, kBoxBytes);
-            ptx::tma_load_2d(ring + lslot * kBoxBytes, &tmapB, (wk + li * p.warps_k) * 64, lrow, bar0 + 8u * lslot);
-        }
-        if (++lslot == p.depth) lslot = 0;
-        if (++li == mine) li = 0, ++lu;
+    // Two walks over (unit, step): loads, and products kDepth steps behind.
+    struct Walk {
+        int left, pair, block, step, expert;
     };
-    // ---- scales two steps ahead: lane (g, q) fetches those of row q * 8 + g and hands them to the lanes that need them
-    using Raw = RawScales<S, GPS>;
-    int su = u_begin, si = 0;
-    const S *sp = nullptr;
-    bool s_ok = false;
-    const int srow = (q % RG) * 8 + g;
-    auto load_scales = [&](Raw &s) {
+    auto advance = [&](Walk &w) {
+        if (++w.step < mine) return;
+        w.step = 0;
+        --w.left;
+        if (++w.block < blocks) return;
+        w.block = 0;
+        ++w.pair;
+        if (p.offsets && w.left > 0) w.expert = expert_of_tile(tiles, p.experts, w.pair);
+    };
+    Walk cw;
+    cw.left = u_end - u_begin, cw.pair = u_begin / blocks, cw.block = u_begin - cw.pair * blocks, cw.step = 0;
+    cw.expert = expert_of(cw.pair);
+    Walk lw = cw;
+
+    struct Step {
+        uint4 w[kRG];
+        RawScales<S, GPS> s;
+    };
+    const uint8_t *lb = nullptr;  // the expert's matrix
+    uint32_t lrow[kRG];           // this lane's rows in it (rows beyond n repeat the last one: nobody reads their sums)
+    const S *sp = nullptr;        // lane (g, q) fetches the scales of row q * 8 + g and hands them to the lanes that need them
+    auto load = [&](Step &b) {
+        if (lw.left <= 0) return;
+        if (lw.step == 0) {
+            const int first = lw.block * block_rows + wr * kRows;
+            lb = p.B + (int64_t)lw.expert * p.n * row_bytes;
 #pragma unroll
-        for (int j = 0; j < Raw::kWords; ++j) s.w[j] = 0;
-        if (su >= u_end) return;
-        if (si == 0) {
-            const int pair = su / blocks, row = (su - pair * blocks) * block_rows + wr * 8 * RG + srow;
-            sp = scales + ((int64_t)expert_of(pair) * p.n + row) * p.groups;
-            s_ok = row < p.n;
+            for (int r = 0; r < kRG; ++r) lrow[r] = (uint32_t)min(first + 8 * r + g, p.n - 1) * row_bytes;
+            sp = scales + ((int64_t)lw.expert * p.n + min(first + q * 8 + g, p.n - 1)) * p.groups;
         }
-        const int t = wk + si * p.warps_k;
-        if (s_ok && t < steps) {
-            const int first = GPS > 1 ? t * GPS : (t * kStep) >> p.group_shift;
-            if constexpr (GPS == 1) {
-                if constexpr (sizeof(S) == 4) s.w[0] = __float_as_uint(to_float(__ldg(sp + first)));
-                else s.w[0] = __ldg(reinterpret_cast<const unsigned short *>(sp + first));
-            } else if (p.vec_scales) {
-                if constexpr (Raw::kWords == 1) s.w[0] = __ldg(reinterpret_cast<const uint32_t *>(sp + first));
-                else if constexpr (Raw::kWords == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(sp + first));
-                    s.w[0] = v.x, s.w[1] = v.y;
-                } else {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(sp + first));
-                    s.w[0] = v.x, s.w[1] = v.y, s.w[2] = v.z, s.w[3] = v.w;
-                }
+        const int t = wk + lw.step * p.warps_k;
+        const uint8_t *src = lb + (4 * t + q < chunks ? t * 64 + q * 16 : 0);  // beyond K the codes meet zeros
+#pragma unroll
+        for (int r = 0; r < kRG; ++r) b.w[r] = __ldcs(reinterpret_cast<const uint4 *>(src + lrow[r]));
+        using Raw = RawScales<S, GPS>;
+        const int first = GPS > 1 ? t * GPS : (t * kStep) >> p.group_shift;
+        if (t >= steps) {
+#pragma unroll
+            for (int j = 0; j < Raw::kWords; ++j) b.s.w[j] = 0;
+        } else if constexpr (GPS == 1) {
+            if constexpr (sizeof(S) == 4) b.s.w[0] = __float_as_uint(to_float(__ldg(sp + first)));
+            else b.s.w[0] = __ldg(reinterpret_cast<const unsigned short *>(sp + first));
+        } else if (p.vec_scales) {
+            if constexpr (Raw::kWords == 1) b.s.w[0] = __ldg(reinterpret_cast<const uint32_t *>(sp + first));
+            else if constexpr (Raw::kWords == 2) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(sp + first));
+                b.s.w[0] = v.x, b.s.w[1] = v.y;
             } else {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(sp + first));
+                b.s.w[0] = v.x, b.s.w[1] = v.y, b.s.w[2] = v.z, b.s.w[3] = v.w;
+            }
+        } else {
 #pragma unroll
-                for (int j = 0; j < GPS; ++j) {
-                    if (first + j >= p.groups) continue;
-                    if constexpr (sizeof(S) == 4) s.w[j] = __float_as_uint(to_float(__ldg(sp + first + j)));
-                    else s.w[j >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(sp + first + j)) << (16 * (j & 1));
-                }
+            for (int j = 0; j < Raw::kWords; ++j) b.s.w[j] = 0;
+#pragma unroll
+            for (int j = 0; j < GPS; ++j) {
+                if (first + j >= p.groups) continue;
+                if constexpr (sizeof(S) == 4) b.s.w[j] = __float_as_uint(to_float(__ldg(sp + first + j)));
+                else b.s.w[j >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(sp + first + j)) << (16 * (j & 1));
             }
         }
-        if (++si == mine) si = 0, ++su;
+        advance(lw);
     };
+    Step buf[kDepth];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) load(buf[d]);
 
-    // Element of a step's 128 at which the eight codes begin that lane (g, q) multiplies in set s (see the trade below).
-    auto set_begin = [&](int s) {
-        if constexpr (GPS == 1) return 32 * q + 8 * s;
-        else if constexpr (GPS == 2) return 32 * (2 * (s >> 1) + (q & 1)) + 8 * (2 * (q >> 1) + (s & 1));
-        else return 32 * s + 8 * q;
-    };
+    unsigned bad_rows = 0;  // rows of X with an element that is not finite, as far as this warp has seen
+    bool staged_bad = false, cpair_seen = false;
+    int parity = 0, pair_parity = 0, first_row = 0, tokens = 0, cpair = -1;
+    float acc[kTiles][4];
 
-    for (int d = 0; d < p.depth; ++d) load_box();
-    Raw raw[2];
-    load_scales(raw[0]);
-    load_scales(raw[1]);
-
-    int cu = u_begin, ci = 0, cslot = 0, cpair = -1, parity = 0;
-    uint32_t phase = 0;
-    bool dead = false;  // a wait gave up: run on without data, so that the block's barriers still meet
-    int first_row = 0, tokens = 0, rb = 0;
-    float acc[kTiles][TT][4];
-
+    // This warp's share of the rows of X as bytes d1, d2, d3.  A lane takes eight elements of a row (side = which row of a pair,
+    // word = which of the step's sixteen eights): the word of codes they will meet is lane (g, q)'s in set s.
     auto stage_x = [&]() {
-        // every lane stores what it will read: the eight elements of each set, in the order of the unpacked codes
-        for (int tt = 0; tt < TT; ++tt) {
-            const int slot = 8 * tt + g;
-            if (slot >= slots) continue;
-            const T *row = X + (int64_t)(first_row + slot) * p.ldx;
-            for (int i = 0; i < mine; ++i) {
+        const int side = lane >> 4, word = lane & 15;
+        const int s = GPS == 1 ? word & 3 : GPS == 2 ? 2 * (word >> 3) + (word & 1) : word >> 2;
+        const int qq = GPS == 1 ? word >> 2 : GPS == 2 ? 2 * ((word >> 1) & 1) + ((word >> 2) & 1) : word & 3;
+        if (groups_of_rows > 1 && cpair_seen) __syncthreads();  // another group may still read the rows before
+        cpair_seen = true;
+        unsigned bad = 0;
+        uint4 v[kTile / 2], ahead[kTile / 2];
+        auto fetch = [&](int i) {
+            const int at = (wk + i * p.warps_k) * kStep + word * 8;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int at = (wk + i * p.warps_k) * kStep + set_begin(s);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (slot < tokens && at < p.k) v = __ldg(reinterpret_cast<const uint4 *>(row + at));
-                    const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                                               __byte_perm(v.y, v.w, 0x7632));  // (0, 4), (1, 5), (2, 6), (3, 7)
-                    if (i < staged) xs[((i * 4 + s) * slots + slot) * 4 + q] = o;
+            for (int r = 0; r < kTile / 2; ++r) {
+                ahead[r] = make_uint4(0, 0, 0, 0);
+                if (i < mine && 2 * r + side < tokens && at < p.k)
+                    ahead[r] = __ldg(reinterpret_cast<const uint4 *>(X + (int64_t)(first_row + 2 * r + side) * p.ldx + at));
+            }
+        };
+        fetch(wr);
+        for (int i = wr; i < mine; i += groups_of_rows) {  // the warp groups share their common steps
+            const int t = wk + i * p.warps_k;
+#pragma unroll
+            for (int r = 0; r < kTile / 2; ++r) v[r] = ahead[r];
+            fetch(i + groups_of_rows);
+#pragma unroll
+            for (int r = 0; r < kTile / 2; ++r) {
+                const int row = 2 * r + side;
+                if (2 * r >= tokens) continue;  // (columns without a row hold anything: nobody reads their sums)
+                uint32_t m = __vmaxu2(__vmaxu2(v[r].x & 0x7FFF7FFFu, v[r].y & 0x7FFF7FFFu), __vmaxu2(v[r].z & 0x7FFF7FFFu, v[r].w & 0x7FFF7FFFu));
+#pragma unroll
+                for (int d = 1; d < 16 / GPS; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+                m = max(m & 0xFFFFu, m >> 16);
+                float top;
+                if constexpr (std::is_same<T, __half>::value) top = __half2float(__ushort_as_half((unsigned short)m));
+                else top = __uint_as_float(m << 16);
+                const uint32_t e = __float_as_uint(top) >> 23;  // biased exponent: top < 2^(e - 126)
+                if (e == 255u) bad |= 1u << row;
+                const uint32_t ec = min(max(e, 25u), 254u);      // (below 2^-101 the bits run out early)
+                const float up = __uint_as_float((274u - ec) << 23);  // 2^21 over the power of two above top
+                uint32_t z[8];
+                const uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float x;
+                    if constexpr (std::is_same<T, __half>::value) x = __half2float(__ushort_as_half((unsigned short)((j & 1) ? w[j >> 1] >> 16 : w[j >> 1])));
+                    else x = __uint_as_float((j & 1) ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
+                    // 1.5 x 2^23 rounds to a whole number; 128 more in the two low digits makes their bytes unsigned
+                    z[j] = __float_as_uint(fmaf(x, up, 12582912.0f + 32896.0f));
+                }
+                // even elements 0, 2, 4, 6 and odd elements 1, 3, 5, 7: their bytes 0 (d3 + 128), 1 (d2 + 128) and 2 (d1 + 64)
+                uint32_t d[3][2];
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const uint32_t a = __byte_perm(z[o], z[2 + o], 0x5140), b = __byte_perm(z[4 + o], z[6 + o], 0x5140);
+                    d[2][o] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+                    d[1][o] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+                    const uint32_t c = __byte_perm(__byte_perm(z[o], z[2 + o], 0x0062), __byte_perm(z[4 + o], z[6 + o], 0x0062), 0x5410);
+                    d[0][o] = ((c | 0x80808080u) - 0x40404040u) ^ 0x80808080u;
+                }
+                const float f = __uint_as_float((ec - 24u) << 23);  // one over up, and over the codes' factor of 16
+                const bool lead = (word & (16 / GPS - 1)) == 0;
+                const int j = GPS == 1 ? 0 : GPS == 2 ? word >> 3 : word >> 2;
+                uint2 *dst = reinterpret_cast<uint2 *>(xs + t * kPlace + (s >> 1) * TT * 32) + (s & 1);
+                float *uf = unit + (t * GPS + j) * kColumns;
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int b = 0; b < 3; ++b) dst[2 * (b * 32 + row * 4 + qq)] = make_uint2(d[b][0], d[b][1]);
+                    if (lead) uf[row] = f;
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 3; ++b) dst[2 * ((2 * b + row) * 4 + qq)] = make_uint2(d[b][0], d[b][1]);
+                    if (lead) uf[row] = f * 65536.0f, uf[2 + row] = f * 256.0f, uf[4 + row] = f, uf[6 + row] = 0.0f;
                 }
             }
         }
+        bad_rows = __reduce_or_sync(0xFFFFFFFFu, bad);
+        pair_parity ^= 1;
+        if (lane == 0) odd_rows[pair_parity * kWarps + warp] = bad_rows;
+        if (groups_of_rows > 1) staged_bad = __syncthreads_or(bad_rows != 0);
+        else __syncwarp();
     };
 
-    auto product = [&](const Raw &raw_scales) {
-        if (!dead && !ptx::warp_wait<false>(bar0 + 8u * cslot, phase, abort_word, lane)) {
-            dead = true;
-            if (lane == 0) tc::report_timeout(p.status, kWaitConvertPacked), *abort_word = 1;
-        }
-        uint4 wv[RG];
-#pragma unroll
-        for (int r = 0; r < RG; ++r) wv[r] = ptx::lds128(ring + cslot * kBoxBytes + r * 512 + lane * 16);
-        if (++cslot == p.depth) cslot = 0, phase ^= 1u;
-        __syncwarp();  // the box is in registers
-        if (!dead) load_box();
+    auto product = [&](Step &b) {
         if constexpr (GPS > 1) {
-            // lanes q and q ^ 2 trade: afterwards sets 0, 1 hold codes of the first 64 elements of the step and sets 2, 3 of the last
+            // lanes q and q ^ 2 trade: afterwards sets 0, 1 hold codes of the first 64 elements and sets 2, 3 of the last
 #pragma unroll
-            for (int r = 0; r < RG; ++r) {
-                uint4 &w = wv[r];
+            for (int r = 0; r < kRG; ++r) {
+                uint4 &w = b.w[r];
                 const bool low = q < 2;
                 const uint32_t s0 = low ? w.z : w.x, s1 = low ? w.w : w.y;
                 const uint32_t r0 = __shfl_xor_sync(0xFFFFFFFFu, s0, 2), r1 = __shfl_xor_sync(0xFFFFFFFFu, s1, 2);
@@ -285,200 +368,171 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
                 }
             }
         }
-        const bool two = TT == 2 && tokens > 8;
-        const bool has0 = g < slots, has1 = 8 + g < slots;
-        float part[kTiles][TT][4];
+        const int t = wk + cw.step * p.warps_k;
+        const uint4 *xp = xs + t * kPlace + lane;
+        const float *uf = unit + t * GPS * kColumns + 2 * q;
+        int sum[kTiles][TT][4];
+        uint4 xv[TT];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-            const uint4 *src = xs + (ci * 4 + s) * slots * 4 + lane;
-            if (has0) x0 = src[0];
-            if (two && has1) x1 = src[32];
+            if (s % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < TT; ++i) xv[i] = xp[((s / 2) * TT + i) * 32];
+            }
             const bool fresh = s % (4 / GPS) == 0;  // a group begins
 #pragma unroll
             for (int tl = 0; tl < kTiles; ++tl) {
-                uint32_t lo[4], hi[4];
-                const uint4 &w0 = wv[2 * tl], &w1 = wv[2 * tl + 1];
-                codes_to_pairs(s == 0 ? w0.x : s == 1 ? w0.y : s == 2 ? w0.z : w0.w, lo, Tag<T>());
-                codes_to_pairs(s == 0 ? w1.x : s == 1 ? w1.y : s == 2 ? w1.z : w1.w, hi, Tag<T>());
-                if (fresh) mma16816<T, true>(part[tl][0], lo[0], hi[0], lo[1], hi[1], x0.x, x0.y);
-                else mma16816<T, false>(part[tl][0], lo[0], hi[0], lo[1], hi[1], x0.x, x0.y);
-                mma16816<T, false>(part[tl][0], lo[2], hi[2], lo[3], hi[3], x0.z, x0.w);
-                if constexpr (TT == 2) {
-                    if (two) {
-                        if (fresh) mma16816<T, true>(part[tl][1], lo[0], hi[0], lo[1], hi[1], x1.x, x1.y);
-                        else mma16816<T, false>(part[tl][1], lo[0], hi[0], lo[1], hi[1], x1.x, x1.y);
-                        mma16816<T, false>(part[tl][1], lo[2], hi[2], lo[3], hi[3], x1.z, x1.w);
-                    }
+                const uint4 &u0 = b.w[2 * tl], &u1 = b.w[2 * tl + 1];
+                const uint32_t w0 = s == 0 ? u0.x : s == 1 ? u0.y : s == 2 ? u0.z : u0.w, w1 = s == 0 ? u1.x : s == 1 ? u1.y : s == 2 ? u1.z : u1.w;
+                // even elements x 16 and odd elements x 16 of rows g and g + 8
+                const uint32_t a0 = (w0 << 4) & 0xF0F0F0F0u, a1 = (w1 << 4) & 0xF0F0F0F0u, a2 = w0 & 0xF0F0F0F0u, a3 = w1 & 0xF0F0F0F0u;
+#pragma unroll
+                for (int i = 0; i < TT; ++i) {
+                    const uint32_t b0 = s % 2 == 0 ? xv[i].x : xv[i].z, b1 = s % 2 == 0 ? xv[i].y : xv[i].w;
+                    if (fresh) mma16832<true>(sum[tl][i], a0, a1, a2, a3, b0, b1);
+                    else mma16832<false>(sum[tl][i], a0, a1, a2, a3, b0, b1);
                 }
             }
-            if ((s + 1) % (4 / GPS) == 0) {  // a group ends: its fp32 sums times its scale
+            if ((s + 1) % (4 / GPS) == 0) {  // a group ends
                 const int j = s / (4 / GPS);
+                const float2 f = *reinterpret_cast<const float2 *>(uf + j * kColumns);
 #pragma unroll
                 for (int tl = 0; tl < kTiles; ++tl) {
-                    const float s0 = scale_at<S, GPS>(raw_scales, j, (lane & 28) | (2 * tl)), s1 = scale_at<S, GPS>(raw_scales, j, (lane & 28) | (2 * tl + 1));
+                    const float s0 = scale_at<S, GPS>(b.s, j, (lane & 28) | (2 * tl)), s1 = scale_at<S, GPS>(b.s, j, (lane & 28) | (2 * tl + 1));
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[tl][0][c] = fmaf(c < 2 ? s0 : s1, part[tl][0][c], acc[tl][0][c]);
-                    if constexpr (TT == 2) {
-                        if (two) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[tl][1][c] = fmaf(c < 2 ? s0 : s1, part[tl][1][c], acc[tl][1][c]);
-                        }
+                    for (int c = 0; c < 4; ++c) {
+                        float v = sum_value(sum[tl][0][c]);
+                        if constexpr (WIDE) v = fmaf(fmaf(v, 256.0f, sum_value(sum[tl][1][c])), 256.0f, sum_value(sum[tl][2][c]));
+                        acc[tl][c] = fmaf(c < 2 ? s0 : s1, v * ((c & 1) ? f.y : f.x), acc[tl][c]);
                     }
                 }
             }
         }
     };
 
+    // the group's 32 x tokens outputs are shared out so that a thread adds up to eight partial sums at a time
+    const int share_bits = (WIDE ? 0 : 2) + (p.warps_k == 16 ? 1 : 0);  // threads per output: the bytes of X (and an idle one), halves of WK
+    const int group_threads = p.warps_k * 32;
     auto reduce_store = [&]() {
         // register c of lane l of tile tl at position (l + 2 tl + (c >> 1)) % 32: writes and reads hit 32 different banks
         float *buffer = red + parity * kRedFloats;
         parity ^= 1;
 #pragma unroll
-        for (int tl = 0; tl < kTiles; ++tl) {
+        for (int tl = 0; tl < kTiles; ++tl)
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    buffer[(((warp * kTiles + tl) * TT + tt) * 4 + c) * 32 + ((lane + 2 * tl + (c >> 1)) & 31)] = acc[tl][tt][c];
-            }
-        }
-        __syncthreads();  // the other buffer may be written after the next one of these: every reader of it is then done
+            for (int c = 0; c < 4; ++c) buffer[((warp * kTiles + tl) * 4 + c) * 32 + ((lane + 2 * tl + (c >> 1)) & 31)] = acc[tl][c];
+        // the other buffer may be written after the next of these barriers: every reader of it is then done
+        const bool any_bad = barrier_or(1 + wr, group_threads, bad_rows != 0) || staged_bad;
         T *out = static_cast<T *>(p.out);
-        for (int o = threadIdx.x; o < block_rows * tokens; o += kThreads) {
-            const int tok = o / block_rows, row = o - tok * block_rows;
-            const int col = rb * block_rows + row;
-            if (col >= p.n) continue;
-            const int ww = row / (8 * RG), r = row - ww * 8 * RG, tl = r >> 4, half = (r >> 3) & 1;
-            const int c = 2 * half + (tok & 1), l = (r & 7) * 4 + ((tok & 7) >> 1);
+        const int todo = tokens << (5 + share_bits);
+        for (int o = (int)threadIdx.x - wr * group_threads; (o & ~31) < todo; o += group_threads) {  // whole warps, for the shuffles
+            const int index = o >> share_bits, part = WIDE ? o : o >> 2, b = o & 3;
+            const int tok = min(index >> 5, kTile - 1), r = index & 31, tl = r >> 4, half = (r >> 3) & 1;
+            const int c = 2 * half + (tok & 1), l = (r & 7) * 4 + (WIDE ? tok >> 1 : b);
+            const float *src = buffer + (((wr * p.warps_k + (p.warps_k == 16 ? (part & 1) * 8 : 0)) * kTiles + tl) * 4 + c) * 32 + ((l + 2 * tl + half) & 31);
             float sum = 0.0f;
-            for (int w = 0; w < p.warps_k; ++w)
-                sum += buffer[((((ww * p.warps_k + w) * kTiles + tl) * TT + (tok >> 3)) * 4 + c) * 32 + ((l + 2 * tl + half) & 31)];
-            out[(int64_t)(first_row + tok) * p.ldo + col] = from_float<T>(sum * kCodeUnit<T>);
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                if (w < p.warps_k) sum += src[w * kTiles * 128];
+            if (!WIDE && b == 3) sum = 0.0f;
+            if constexpr (!WIDE) {
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+            }
+            if (p.warps_k == 16) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, WIDE ? 1 : 4);
+            const int col = cw.block * block_rows + wr * kRows + r;
+            if (o >= todo || (o & ((1 << share_bits) - 1)) != 0 || col >= p.n) continue;
+            if (any_bad) {
+                unsigned bad = 0;
+                for (int w = 0; w < kWarps; ++w) bad |= odd_rows[pair_parity * kWarps + w];
+                if (bad >> tok & 1) {
+                    const int64_t brow = (int64_t)cw.expert * p.n + col;
+                    sum = plain_output(X + (int64_t)(first_row + tok) * p.ldx, p.B + brow * (p.k / 2), scales + brow * p.groups, p.k, 1 << p.group_shift);
+                }
+            }
+            out[(int64_t)(first_row + tok) * p.ldo + col] = from_float<T>(sum);
         }
     };
 
     for (;;) {
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            if (ci == 0) {
-                if (cu >= u_end) return;
-                const int pair = cu / blocks;
-                rb = cu - pair * blocks;
-                if (pair != cpair) {
-                    cpair = pair;
+        for (int d = 0; d < kDepth; ++d) {
+            if (cw.step == 0) {
+                if (cw.left <= 0) return;
+                if (cw.pair != cpair) {
+                    cpair = cw.pair;
                     if (p.offsets) {
-                        const int e = expert_of(pair);
-                        first_row = seg[e] + (pair - tiles[e]) * p.tile;
-                        tokens = min(p.tile, seg[e + 1] - first_row);
+                        first_row = seg[cw.expert] + (cw.pair - tiles[cw.expert]) * kTile;
+                        tokens = min(kTile, seg[cw.expert + 1] - first_row);
                     } else {
-                        first_row = pair * p.tile;
-                        tokens = min(p.tile, p.rows - first_row);
+                        first_row = cw.pair * kTile;
+                        tokens = min(kTile, p.rows - first_row);
                     }
                     stage_x();
                 }
 #pragma unroll
                 for (int tl = 0; tl < kTiles; ++tl)
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) acc[tl][tt][c] = 0.0f;
+                    for (int c = 0; c < 4; ++c) acc[tl][c] = 0.0f;
             }
-            product(raw[d]);
-            load_scales(raw[d]);
-            if (++ci == mine) {
-                ci = 0, ++cu;
-                reduce_store();
-            }
+            product(buf[d]);
+            load(buf[d]);
+            if (cw.step == mine - 1) reduce_store();
+            advance(cw);
         }
     }
 }
 
-int log2_of(int v)
-{
-    int s = 0;
-    while ((1 << s) < v) ++s;
-    return s;
-}
-
 struct RowsPlan {
-    int tile, warps_k, rg, depth;
+    bool wide;
+    int warps_k;
     size_t smem;
 };
 
-size_t rows_smem(int k, const RowsPlan &p, int experts)
-{
-    const int steps = (k + kStep - 1) / kStep, staged = (steps + p.warps_k - 1) / p.warps_k;
-    return (size_t)kWarps * p.depth * 512 * p.rg + (size_t)kWarps * staged * 4 * p.tile * 64 + 2 * (size_t)kWarps * (p.rg / 2) * (p.tile > 8 ? 2 : 1) * 512 +
-           kWarps * kMaxDepth * 8 + 8 + (size_t)(experts + 1) * 8;
-}
-
-// false: the staged rows of X do not fit
+// false: X does not fit
 bool rows_plan(const W4Args &a, int sms, RowsPlan *plan)
 {
     RowsPlan p;
     const int steps = (a.k + kStep - 1) / kStep;
-    // warps beyond the steps of K would idle: they take further rows of B instead
-    p.warps_k = steps >= 12 ? 16 : steps >= 6 ? 8 : 4;
-    p.tile = a.offsets ? 16 : (a.rows < 16 ? a.rows : 16);
-    p.rg = 4;
-    (void)sms;
-    // the deepest ring that leaves room for X; two boxes a warp are the least that keeps the stream going
-    auto fit = [&]() {
-        for (p.depth = kMaxDepth; p.depth >= 2; --p.depth)
-            if (rows_smem(a.k, p, a.experts) <= (size_t)kMaxSmem) return true;
-        return false;
-    };
-    bool ok = fit();
-    if (!ok && p.tile > 8) {
-        p.tile = 8;
-        ok = fit();
-    }
-    if (ok) p.smem = rows_smem(a.k, p, a.experts);
+    p.wide = a.offsets ? a.rows > (a.experts < a.rows ? a.experts : a.rows) : a.rows > kNarrowRows;
+    // Warps that split K: all, or as many as there are steps.  Only where a CTA has many blocks to do, and the block's end is long (WIDE),
+    // warp groups that take turns at it pay: 4096 units over 148 CTAs (27 each), 8 rows, 4096 x 4096: 84 us with WK = 16, 71 with 4;
+    // 896 units (6 each): 35.0 against 37.4; 1792 units of one row: 55.6 against 64.7.
+    const int tile = p.wide ? kWideRows : kNarrowRows;
+    const int64_t pairs = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : (a.rows + tile - 1) / tile;  // (with experts: at most)
+    const int64_t units = pairs * ((a.n + kRows - 1) / kRows);
+    p.warps_k = (p.wide && units >= 16 * (int64_t)sms) || steps <= 4 ? 4 : steps <= 8 ? 8 : 16;
+    const int places = steps > p.warps_k ? steps : p.warps_k, gps = a.group >= kStep ? 1 : kStep / a.group;
+    p.smem = (size_t)places * ((p.wide ? 3 : 1) * 1024 + gps * 32) + 2 * (size_t)kRedFloats * 4 + 2 * kWarps * 4 + (size_t)(a.experts + 1) * 8;
     *plan = p;
-    return ok;
+    return p.smem <= (size_t)kMaxSmem;
 }
 
-template <typename T, typename S, int GPS, int RG, int TT>
+template <typename T, typename S, int GPS, bool WIDE>
 int rows_launch_variant(const W4Args &a, const RowsPlan &plan, const DeviceCtx &ctx)
 {
-    auto kernel = w4_rows_kernel<T, S, GPS, RG, TT>;
+    auto kernel = w4_rows_kernel<T, S, GPS, WIDE>;
     static std::atomic<bool> configured[64];  // set once per device; a repeated cudaFuncSetAttribute is harmless
     if (!configured[ctx.device & 63].load(std::memory_order_acquire)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
         if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(w4_rows_kernel)");
         configured[ctx.device & 63].store(true, std::memory_order_release);
     }
-    CUtensorMap tmB;
-    int st = tc::make_packed_tmap(&tmB, a.B, a.experts * a.n, a.k / 2, 8 * RG, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (st != QM_OK) return st;
     RowsParams p;
-    p.depth = plan.depth, p.status = ctx.status;
-    p.X = a.X, p.ldx = a.ldx, p.scales = a.scales, p.offsets = a.offsets, p.out = a.out, p.ldo = a.ldo;
+    p.X = a.X, p.ldx = a.ldx, p.B = a.B, p.scales = a.scales, p.offsets = a.offsets, p.out = a.out, p.ldo = a.ldo;
     p.rows = a.rows, p.n = a.n, p.k = a.k, p.experts = a.experts;
-    p.group_shift = log2_of(a.group), p.groups = (a.k + a.group - 1) / a.group;
-    p.tile = plan.tile, p.warps_k = plan.warps_k;
+    p.group_shift = a.group == 32 ? 5 : a.group == 64 ? 6 : a.group == 128 ? 7 : 8;
+    p.groups = (a.k + a.group - 1) / a.group;
+    p.warps_k = plan.warps_k;
     // a step's scales lie on a boundary of their own size when a row has a multiple of GPS of them
-    p.vec_scales = p.groups % GPS == 0 && (reinterpret_cast<uintptr_t>(a.scales) & (GPS * sizeof(S) - 1)) == 0;
-    const int block_rows = 8 * RG * (kWarps / plan.warps_k);
+    p.vec_scales = p.groups % GPS == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 15u) == 0;
+    const int block_rows = kRows * (kWarps / plan.warps_k), tile = WIDE ? kWideRows : kNarrowRows;
     const int64_t blocks = (a.n + block_rows - 1) / block_rows;
     // with experts the units are known on the device only: at most one tile more than whole ones per expert that can have rows
-    const int64_t pairs = a.offsets ? a.rows / plan.tile + (a.experts < a.rows ? a.experts : a.rows) : (a.rows + plan.tile - 1) / plan.tile;
+    const int64_t pairs = a.offsets ? a.rows / tile + (a.experts < a.rows ? a.experts : a.rows) : (a.rows + tile - 1) / tile;
     const int64_t units = pairs * blocks;
     if (units > 0x7FFFFFFF) return QM_ERR_SHAPE;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units < ctx.num_sms ? units : ctx.num_sms), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = plan.smem;
-    cfg.stream = a.stream;
-    cudaLaunchAttribute attr[1];
-    static const bool allow_pdl = !std::getenv("QM_NO_PDL");
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = allow_pdl ? 1 : 0;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmB, p);
-    return e == cudaSuccess ? QM_OK : record_cuda_error(e, "w4_rows_kernel launch");
+    return launch_chained("w4_rows_kernel launch", kernel, (unsigned)(units < ctx.num_sms ? units : ctx.num_sms), kThreads, plan.smem, a.stream, p);
 }
 
 }  // namespace
@@ -486,8 +540,9 @@ int rows_launch_variant(const W4Args &a, const RowsPlan &plan, const DeviceCtx &
 bool w4_rows_eligible(const W4Args &a, const DeviceCtx &ctx)
 {
     RowsPlan plan;
-    return a.k > 0 && a.k % 32 == 0 && a.ldx % 8 == 0 && (int64_t)a.experts * a.n <= 0x7FFFFFFF - 512 && ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.B)) & 15u) == 0 &&
-           rows_plan(a, ctx.num_sms, &plan);
+    const int sms = ctx.num_sms;
+    return a.k > 0 && a.k % 32 == 0 && a.ldx % 8 == 0 && (int64_t)a.n * (a.k / 2) < (1ll << 32) &&
+           ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.B)) & 15u) == 0 && rows_plan(a, sms, &plan);
 }
 
 int w4_rows_launch(const W4Args &a, const DeviceCtx &ctx)
@@ -498,13 +553,13 @@ int w4_rows_launch(const W4Args &a, const DeviceCtx &ctx)
         using T = typename decltype(t)::type;
         return with_same_or_float<T>(a.scale_type, [&](auto u) {
             using S = typename decltype(u)::type;
-            auto by_group = [&](auto tt) {
-                constexpr int TT = decltype(tt)::value;
-                if (a.group == 32) return rows_launch_variant<T, S, 4, 4, TT>(a, plan, ctx);
-                if (a.group == 64) return rows_launch_variant<T, S, 2, 4, TT>(a, plan, ctx);
-                return rows_launch_variant<T, S, 1, 4, TT>(a, plan, ctx);
+            auto by_group = [&](auto wide) {
+                constexpr bool WIDE = decltype(wide)::value;
+                if (a.group == 32) return rows_launch_variant<T, S, 4, WIDE>(a, plan, ctx);
+                if (a.group == 64) return rows_launch_variant<T, S, 2, WIDE>(a, plan, ctx);
+                return rows_launch_variant<T, S, 1, WIDE>(a, plan, ctx);
             };
-            return plan.tile > 8 ? by_group(std::integral_constant<int, 2>()) : by_group(std::integral_constant<int, 1>());
+            return plan.wide ? by_group(std::true_type()) : by_group(std::false_type());
         });
     };
     return a.type == QM_TYPE_F16 ? by_type(Tag<__half>()) : by_type(Tag<__nv_bfloat16>());

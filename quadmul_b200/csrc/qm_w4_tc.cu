@@ -71,22 +71,6 @@ struct TcParams {
     int *status;
 };
 
-// One lane of the (converged) warp, always the same one.  The code around it stays uniform over the warp, so that the compiler
-// keeps descriptors and addresses in uniform registers, which is where tcgen05.mma takes them: issued from a divergent branch
-// an MMA cost 85 clocks, most of them moves.
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t r;
-    asm volatile(
-        "{\n"
-        " .reg .pred p;\n"
-        " elect.sync _|p, 0xFFFFFFFF;\n"
-        " selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(r));
-    return r != 0;
-}
-
 // D[tmem] (+)= A[tmem] * B[smem desc], 16-bit floats -> fp32.  One thread issues it.
 template <int G>
 __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
