@@ -5,7 +5,8 @@
 // Sorting.  slot(t, j) = (assignments to lower experts) + (earlier assignments to the same expert): a counting sort, stable, without
 // atomics on anything that decides an order.  Up to kFewIds assignments take ONE launch: every block counts all ids itself
 // (they are L2 hits), which saves two launches and a workspace.  More take three: counts per block of assignments, a scan of
-// the counts over the blocks, and the placing.
+// the counts over the blocks, and the placing.  With up to 64 experts ids are counted without atomics: a lane has the counts of
+// one or two experts in registers, and finds who of 32 ids names them from a ballot per bit of the id.
 #include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
@@ -15,9 +16,10 @@ using namespace w4;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kFewIds = 2048;
-constexpr int kBlocks = 148 * 4;  // blocks that share the assignments
+constexpr int kThreads = 256;       // of the sums and their gradients
+constexpr int kSortThreads = 1024;
+constexpr int kFewIds = 16384;
+constexpr int kFewBlocks = 148, kManyBlocks = 148 * 2;  // blocks that share the assignments
 
 // VEC elements of T that move together: 16 bytes, or one element where rows are not on 16-byte boundaries.
 template <typename T, int VEC>
@@ -38,19 +40,16 @@ struct Piece {
 
 __device__ __forceinline__ int expert_id(int64_t id, int experts) { return id >= 0 && id < experts ? (int)id : -1; }
 
-// Adds each lane's expert (-1: none) to counts[]: one atomic per expert of the warp.
-__device__ __forceinline__ void count_ids(int *counts, int e, int lane)
-{
-    const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + e, __popc(same));
-}
-
-// Ids [first, last) -> how many go to each expert, in counts[0 .. experts); the whole block.
+// Ids [first, last) -> how many go to each expert, added to counts[0 .. experts) in shared memory; the whole block.
 template <typename I>
 __device__ __forceinline__ void count_range(const I *__restrict__ ids, int64_t first, int64_t last, int experts, int *counts)
 {
+    constexpr int kAhead = 8;  // loads in flight
     const int lane = threadIdx.x & 31;
-    constexpr int kAhead = 4;  // loads in flight
+    int mine[2] = {0, 0};  // of experts lane and lane + 32
+    unsigned flip[5];      // bit b of a lane's expert: who has another one
+#pragma unroll
+    for (int b = 0; b < 5; ++b) flip[b] = (lane >> b) & 1 ? 0u : 0xFFFFFFFFu;
     for (int64_t base = first + (threadIdx.x & ~31); base < last; base += kAhead * (int64_t)blockDim.x) {
         int e[kAhead];
 #pragma unroll
@@ -59,23 +58,39 @@ __device__ __forceinline__ void count_range(const I *__restrict__ ids, int64_t f
             e[u] = i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1;
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) count_ids(counts, e[u], lane);
+        for (int u = 0; u < kAhead; ++u) {
+            if (base + u * (int64_t)blockDim.x >= last) break;  // uniform over the warp
+            if (experts <= 64) {
+                unsigned same = __ballot_sync(0xFFFFFFFFu, e[u] >= 0);
+#pragma unroll
+                for (int b = 0; b < 5; ++b) same &= __ballot_sync(0xFFFFFFFFu, (e[u] >> b) & 1) ^ flip[b];
+                const unsigned high = __ballot_sync(0xFFFFFFFFu, e[u] & 32);
+                mine[0] += __popc(same & ~high);
+                mine[1] += __popc(same & high);
+            } else if (e[u] >= 0) {
+                atomicAdd(counts + e[u], 1);
+            }
+        }
+    }
+    if (experts <= 64) {
+        if (lane < experts && mine[0]) atomicAdd(counts + lane, mine[0]);
+        if (lane + 32 < experts && mine[1]) atomicAdd(counts + lane + 32, mine[1]);
     }
 }
 
 // counts[block][expert] of the block's assignments
 template <typename I>
-__global__ void __launch_bounds__(kThreads) moe_count_kernel(const I *__restrict__ ids, int experts, int count, int per_block, int *__restrict__ counts)
+__global__ void __launch_bounds__(kSortThreads) moe_count_kernel(const I *__restrict__ ids, int experts, int count, int per_block, int *__restrict__ counts)
 {
     extern __shared__ int mine[];
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
-    for (int e = threadIdx.x; e < experts; e += kThreads) mine[e] = 0;
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) mine[e] = 0;
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * per_block;
     count_range(ids, first, min((int64_t)count, first + per_block), experts, mine);
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kThreads) counts[(int64_t)blockIdx.x * experts + e] = mine[e];
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) counts[(int64_t)blockIdx.x * experts + e] = mine[e];
 }
 
 // counts[block][expert] -> how many earlier blocks have, totals[expert]; one warp per expert
@@ -103,22 +118,23 @@ __global__ void __launch_bounds__(kThreads) moe_scan_kernel(int *__restrict__ co
 
 // Slots of the block's tokens and the copy of their rows.  counts == NULL: the block counts all ids itself.
 template <typename T, typename I, int VEC>
-__global__ void __launch_bounds__(kThreads) moe_place_kernel(const T *__restrict__ X, int64_t ldx, const I *__restrict__ ids, int experts, int tokens,
+__global__ void __launch_bounds__(kSortThreads) moe_place_kernel(const T *__restrict__ X, int64_t ldx, const I *__restrict__ ids, int experts, int tokens,
                                                              int top_k, int hidden, int per_block, const int *__restrict__ counts,
                                                              const int *__restrict__ totals, T *__restrict__ xs, int64_t ldxs, int *__restrict__ offsets,
                                                              int *__restrict__ slots)
 {
     extern __shared__ int smem[];
-    int *next = smem, *total = smem + experts, *at = total + experts;  // at: the slots of the block's assignments
+    int *next = smem, *total = smem + experts, *at = total + experts;  // at: the experts, then the slots of the block's assignments
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const int64_t first = (int64_t)blockIdx.x * per_block * top_k;
     const int64_t last = min((int64_t)tokens * top_k, first + (int64_t)per_block * top_k);
-    for (int e = threadIdx.x; e < experts; e += kThreads) {
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) {
         next[e] = counts ? counts[(int64_t)blockIdx.x * experts + e] : 0;
         total[e] = counts ? totals[e] : 0;
     }
+    for (int i = threadIdx.x; i < (int)(last - first); i += kSortThreads) at[i] = expert_id((int64_t)__ldg(ids + first + i), experts);
     __syncthreads();
     if (!counts) {
         count_range(ids, 0, first, experts, next);
@@ -146,18 +162,18 @@ __global__ void __launch_bounds__(kThreads) moe_place_kernel(const T *__restrict
         if (blockIdx.x == 0 && lane == 0) offsets[experts] = sum;
         __syncwarp();
         // the block's assignments in order, 32 at a time; lanes with the same expert are ranked by a match
-        for (int64_t base = first; base < last; base += 32) {
-            const int64_t i = base + lane;
-            const int e = i < last ? expert_id((int64_t)__ldg(ids + i), experts) : -1;
+        for (int base = 0; base < (int)(last - first); base += 32) {
+            const int i = base + lane;
+            const int e = i < (int)(last - first) ? at[i] : -1;
             const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
             const int rank = __popc(same & ((1u << lane) - 1u));
             const int slot = e >= 0 ? next[e] + rank : -1;
             __syncwarp();
             if (e >= 0 && rank == 0) next[e] += __popc(same);
             __syncwarp();
-            if (i < last) {
-                slots[i] = slot;
-                at[i - first] = slot;
+            if (i < (int)(last - first)) {
+                slots[first + i] = slot;
+                at[i] = slot;
             }
         }
     }
@@ -166,25 +182,26 @@ __global__ void __launch_bounds__(kThreads) moe_place_kernel(const T *__restrict
     const int pieces = hidden / VEC;
     const int block_tokens = top_k > 0 ? (int)((last - first) / top_k) : 0;
     // the block's (token, piece) pairs are dealt to its threads
-    constexpr int kAhead = 4;
-    const int todo = block_tokens * pieces;  // at most kMaxSlots tokens
-    for (int base = threadIdx.x; base < todo; base += kAhead * kThreads) {
+    constexpr int kAhead = VEC == 1 ? 8 : 4;
+    const int step_t = kSortThreads / pieces, step_c = kSortThreads - step_t * pieces;  // (a division per piece costs more than the copy)
+    int t = (int)threadIdx.x / pieces, c = (int)threadIdx.x - t * pieces;
+    while (t < block_tokens) {
         Piece<T, VEC> v[kAhead];
-        int t[kAhead], c[kAhead];
+        int tt[kAhead], cc[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int i = base + u * kThreads;
-            t[u] = i < todo ? i / pieces : -1;
-            if (t[u] < 0) continue;
-            c[u] = (i - t[u] * pieces) * VEC;
-            v[u].load(X + ((int64_t)blockIdx.x * per_block + t[u]) * ldx + c[u]);
+            tt[u] = t, cc[u] = c * VEC;
+            if (t < block_tokens) v[u].load(X + ((int64_t)blockIdx.x * per_block + t) * ldx + cc[u]);
+            t += step_t, c += step_c;
+            if (c >= pieces) c -= pieces, ++t;
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (t[u] < 0) continue;
+            if (tt[u] >= block_tokens) continue;
+            T *dst = xs + cc[u];
             for (int j = 0; j < top_k; ++j) {
-                const int slot = at[t[u] * top_k + j];
-                if (slot >= 0) v[u].store(xs + (int64_t)slot * ldxs + c[u]);
+                const int slot = at[tt[u] * top_k + j];
+                if (slot >= 0) v[u].store(dst + (int64_t)slot * ldxs);
             }
         }
     }
@@ -198,15 +215,18 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
 {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
-    constexpr int kAhead = 8;  // rows in flight per thread
+    constexpr int kAhead = 8;                // rows in flight per thread
+    constexpr int kCols = VEC == 1 ? 4 : 1;  // pieces of a row per thread and turn: single elements need more of them in flight
     const int64_t t = blockIdx.x / parts;
     const int part = (int)(blockIdx.x % parts);
-    for (int c = (part * kThreads + (int)threadIdx.x) * VEC; c < hidden; c += parts * kThreads * VEC) {
-        float sum[VEC];
+    for (int c0 = (part * kThreads * kCols + (int)threadIdx.x) * VEC; c0 < hidden; c0 += parts * kThreads * kCols * VEC) {
+        float sum[kCols][VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+        for (int o = 0; o < kCols; ++o)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[o][i] = 0.0f;
         for (int j0 = 0; j0 < top_k; j0 += kAhead) {
-            Piece<T, VEC> v[kAhead];
+            Piece<T, VEC> v[kAhead][kCols];
             float w[kAhead];
             bool live[kAhead];
 #pragma unroll
@@ -217,19 +237,27 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
                 live[j] = at >= 0 && at < rows;
                 if (!live[j]) continue;
                 w[j] = weights ? to_float(__ldg(weights + t * top_k + j0 + j)) : 1.0f;
-                v[j].load(ys + (int64_t)at * ldys + c);
+#pragma unroll
+                for (int o = 0; o < kCols; ++o)
+                    if (c0 + o * kThreads * VEC < hidden) v[j][o].load(ys + (int64_t)at * ldys + c0 + o * kThreads * VEC);
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (!live[j]) continue;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) sum[i] = fmaf(w[j], to_float(v[j].v[i]), sum[i]);
+                for (int o = 0; o < kCols; ++o)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) sum[o][i] = fmaf(w[j], to_float(v[j][o].v[i]), sum[o][i]);
             }
         }
-        Piece<T, VEC> o;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o.v[i] = from_float<T>(sum[i]);
-        o.store(y + t * ldy + c);
+        for (int o = 0; o < kCols; ++o) {
+            if (c0 + o * kThreads * VEC >= hidden) continue;
+            Piece<T, VEC> r;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) r.v[i] = from_float<T>(sum[o][i]);
+            r.store(y + t * ldy + c0 + o * kThreads * VEC);
+        }
     }
 }
 
@@ -256,6 +284,7 @@ __global__ void __launch_bounds__(kThreads) moe_combine_grad_kernel(const T *__r
             w[j] = at[j] >= 0 ? to_float(__ldg(weights + t * top_k + j0 + j)) : 0.0f;
             dot[j] = 0.0f;
         }
+#pragma unroll(VEC == 1 ? 4 : 1)
         for (int c = (int)threadIdx.x * VEC; c < hidden; c += kThreads * VEC) {
             Piece<T, VEC> d, v[kAhead];
             d.load(dy + t * lddy + c);
@@ -305,7 +334,8 @@ constexpr int kMaxSlots = 8192;  // slots a block keeps in shared memory; top_k 
 
 int tokens_per_block(int tokens, int top_k)
 {
-    const int per = (tokens + kBlocks - 1) / kBlocks, most = kMaxSlots / (top_k > 0 ? top_k : 1);
+    const int blocks = (int64_t)tokens * top_k <= kFewIds ? kFewBlocks : kManyBlocks;
+    const int per = (tokens + blocks - 1) / blocks, most = kMaxSlots / (top_k > 0 ? top_k : 1);
     return per < 1 ? 1 : per < most ? per : most;
 }
 
@@ -330,7 +360,7 @@ int moe_sort_launch(const MoeSortArgs &a)
         if (count > kFewIds) {
             totals = a.workspace;
             counts = a.workspace + a.experts;
-            int st = launch_chained("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kThreads, (size_t)a.experts * sizeof(int), a.stream, ids,
+            int st = launch_chained("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kSortThreads, (size_t)a.experts * sizeof(int), a.stream, ids,
                                     a.experts, count, per * a.top_k, counts);
             if (st != QM_OK) return st;
             st = launch_chained("moe_scan_kernel launch", moe_scan_kernel, (unsigned)((a.experts + 7) / 8), kThreads, 0, a.stream, counts, totals, a.experts,
@@ -347,7 +377,7 @@ int moe_sort_launch(const MoeSortArgs &a)
                     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(moe_place_kernel)");
                 }
-                return launch_chained("moe_place_kernel launch", kernel, (unsigned)blocks, kThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
+                return launch_chained("moe_place_kernel launch", kernel, (unsigned)blocks, kSortThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
                                       a.experts, a.tokens, a.top_k, a.hidden, per, (const int *)counts, (const int *)totals, static_cast<T *>(a.xs), a.ldxs,
                                       a.offsets, a.slots);
             });
@@ -366,7 +396,8 @@ int moe_combine_launch(const MoeCombineArgs &a)
             return with_pieces<T>(vec, [&](auto v) {
                 constexpr int VEC = decltype(v)::value;
                 // a thread per piece while the grid allows it
-                int64_t parts = (a.hidden + kThreads * VEC - 1) / (kThreads * VEC);
+                constexpr int kStretch = kThreads * (VEC == 1 ? 4 : VEC);
+                int64_t parts = (a.hidden + kStretch - 1) / kStretch;
                 if (parts * a.tokens > 0x7FFFFFFF) parts = 1;
                 return launch_chained("moe_combine_kernel launch", moe_combine_kernel<T, S, VEC>, (unsigned)(parts * a.tokens), kThreads, 0, a.stream,
                                       static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots, static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo,
