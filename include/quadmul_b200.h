@@ -281,10 +281,16 @@ typedef enum qm_type {
 /*
  * X (m x k, row pitch ldx elements) times the transpose of B into out (m x n, row pitch ldo elements); X and out are both
  * QM_TYPE_F16 or both QM_TYPE_BF16 (`type`), the scales have that type or QM_TYPE_F32, group is 32, 64, 128 or 256, k is even.
- * Sums are fp32 and are rounded to `type` once.  out is fully overwritten; k == 0 zeroes it.
+ * Sums are fp32 and are rounded to `type` once; with many rows a weight scale * q is rounded to `type` before it is multiplied
+ * (fp16: relative to the largest scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).  A scale
+ * that is not finite makes its column not finite.  out is fully overwritten; k == 0 zeroes it.  n * experts is below 2^31 - 512.
+ *   k % 32 == 0, ldx % 8 == 0 and 16-byte-aligned X and B need no workspace.  Otherwise X and B are copied into one (device
+ *   memory, 16-byte aligned) with k rounded up to 32; qm_gemm_w4_workspace_bytes says how many bytes (experts = 1 for qm_gemm_w4),
+ *   QM_ERR_WORKSPACE if there are fewer.
  */
 int qm_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group, void *out,
-               int64_t ldo, int m, int n, int k, void *stream);
+               int64_t ldo, int m, int n, int k, void *workspace, size_t workspace_bytes, void *stream);
+size_t qm_gemm_w4_workspace_bytes(const void *X, int64_t ldx, const void *B, int experts, int rows, int n, int k);
 
 /*
  * The same product with one weight matrix per expert, over rows that are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1
@@ -293,7 +299,8 @@ int qm_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *
  * captured.  experts is at most 4096.  Offsets outside [0, rows] are clamped; rows of out that belong to no expert are left as they were.
  */
 int qm_moe_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group,
-                   const int *offsets, int experts, void *out, int64_t ldo, int rows, int n, int k, void *stream);
+                   const int *offsets, int experts, void *out, int64_t ldo, int rows, int n, int k, void *workspace,
+                   size_t workspace_bytes, void *stream);
 
 /*
  * W (rows x k, row pitch ldw elements, any qm_type_t) -> packed codes (rows x k/2 bytes) and scales (rows x ceil(k / group),

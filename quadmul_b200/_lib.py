@@ -60,8 +60,9 @@ SIGNATURES = {
     "qm_prelayout_b_bytes": (ctypes.c_size_t, [_i, _i]),
     "qm_prelayout_b": (_i, [_vp, _vp, _i, _i, _vp]),
     "qm_gemm_s4_prelaid": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
-    "qm_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i64, _i, _i, _i, _vp]),
-    "qm_moe_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
+    "qm_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i64, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
+    "qm_gemm_w4_workspace_bytes": (ctypes.c_size_t, [_vp, _i64, _vp, _i, _i, _i, _i]),
+    "qm_moe_gemm_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
     "qm_quantize_w4": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i64, _i64, _i, _vp]),
     "qm_moe_sort": (_i, [_vp, _i, _i64, _vp, _i, _i, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
     "qm_moe_sort_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),

@@ -14,7 +14,7 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libquadmul_b200.so")
-SOURCES = ["qm_api.cu", "qm_gemm_tc.cu", "qm_gemm_tc2.cu", "qm_gemm_dec.cu", "qm_gemv.cu", "qm_gemm_rmma.cu", "qm_gemm_simt.cu", "qm_pack.cu", "qm_dequant.cu", "qm_static_scratch.cu", "qm_peer_flags.cu", "qm_api_w4.cu", "qm_w4_simt.cu", "qm_w4_rows.cu", "qm_w4_tc.cu", "qm_w4_quant.cu", "qm_moe.cu"]
+SOURCES = ["qm_api.cu", "qm_gemm_tc.cu", "qm_gemm_tc2.cu", "qm_gemm_dec.cu", "qm_gemv.cu", "qm_gemm_rmma.cu", "qm_gemm_simt.cu", "qm_pack.cu", "qm_dequant.cu", "qm_static_scratch.cu", "qm_peer_flags.cu", "qm_api_w4.cu", "qm_w4_pad.cu", "qm_w4_rows.cu", "qm_w4_tc.cu", "qm_w4_quant.cu", "qm_moe.cu"]
 HEADERS = ["qm_internal.h", "qm_ptx.cuh", "qm_tile_table.h", "qm_tc_common.cuh", "qm_epilogue.cuh", "qm_w4.cuh", "tile_table.inc", os.path.join("..", "..", "include", "quadmul_b200.h")]
 
 

@@ -20,22 +20,26 @@ int check_w4(const W4Args &a)
     if (!known_group(a.group)) return QM_ERR_ARG;
     if (a.rows == 0 || a.n == 0) return QM_OK;
     if (!a.out || (a.k > 0 && (!a.X || (a.experts > 0 && (!a.B || !a.scales))))) return QM_ERR_NULL;
-    if (a.ldo < a.n || a.ldx < a.k) return QM_ERR_SHAPE;
+    if (a.ldo < a.n || a.ldx < a.k || (int64_t)a.experts * a.n > INT_MAX - 512) return QM_ERR_SHAPE;
     if (!aligned_to(a.X, 2) || !aligned_to(a.out, 2) || !aligned_to(a.scales, w4::type_bytes(a.scale_type))) return QM_ERR_ALIGN;
     return QM_OK;
 }
 
-int w4_dispatch(const W4Args &a)
+int w4_dispatch(W4Args a, void *workspace, size_t workspace_bytes)
 {
     int st = check_w4(a);
     if (st != QM_OK || a.rows == 0 || a.n == 0 || a.experts == 0) return st;
+    const size_t need = w4_workspace(a);
+    if (need && (!workspace || workspace_bytes < need)) return QM_ERR_WORKSPACE;
+    if (need && !aligned_to(workspace, 16)) return QM_ERR_ALIGN;
     DeviceCtx *ctx = nullptr;
     st = device_ctx(&ctx);
     if (st != QM_OK) return st;
+    if (a.k == 0) return w4_zero_launch(a);
+    if (need && (st = w4_pad_launch(&a, workspace)) != QM_OK) return st;
     const int average = a.rows / (a.experts < a.rows ? a.experts : a.rows);
     if (average <= 8 && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
-    if (w4_tc_eligible(a)) return w4_tc_launch(a, *ctx);
-    return w4_simt_launch(a);
+    return w4_tc_launch(a, *ctx);
 }
 
 int check_moe(int type, int tokens, int top_k, int hidden)
@@ -49,19 +53,28 @@ int check_moe(int type, int tokens, int top_k, int hidden)
 extern "C" {
 
 int qm_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group, void *out, int64_t ldo, int m,
-               int n, int k, void *stream)
+               int n, int k, void *workspace, size_t workspace_bytes, void *stream)
 {
     return w4_dispatch({X, type, ldx, static_cast<const uint8_t *>(B), scales, scale_type, group, nullptr, 1, out, ldo, m, n, k,
-                        static_cast<cudaStream_t>(stream)});
+                        static_cast<cudaStream_t>(stream)},
+                       workspace, workspace_bytes);
 }
 
 int qm_moe_gemm_w4(const void *X, int type, int64_t ldx, const void *B, const void *scales, int scale_type, int group, const int *offsets,
-                   int experts, void *out, int64_t ldo, int rows, int n, int k, void *stream)
+                   int experts, void *out, int64_t ldo, int rows, int n, int k, void *workspace, size_t workspace_bytes, void *stream)
 {
     if (!offsets) return QM_ERR_NULL;
     if (!aligned_to(offsets, 4)) return QM_ERR_ALIGN;
     return w4_dispatch({X, type, ldx, static_cast<const uint8_t *>(B), scales, scale_type, group, offsets, experts, out, ldo, rows, n, k,
-                        static_cast<cudaStream_t>(stream)});
+                        static_cast<cudaStream_t>(stream)},
+                       workspace, workspace_bytes);
+}
+
+size_t qm_gemm_w4_workspace_bytes(const void *X, int64_t ldx, const void *B, int experts, int rows, int n, int k)
+{
+    W4Args a = {};
+    a.X = X, a.ldx = ldx, a.B = static_cast<const uint8_t *>(B), a.experts = experts, a.rows = rows, a.n = n, a.k = k;
+    return w4_workspace(a);
 }
 
 int qm_quantize_w4(const void *W, int type, int64_t ldw, void *packed, void *scales, int scale_type, int64_t rows, int64_t k, int group, void *stream)

@@ -146,13 +146,15 @@ struct W4Args {
     int rows, n, k;
     cudaStream_t stream;
 };
-int w4_simt_launch(const W4Args &a);  // qm_w4_simt.cu
+// qm_w4_pad.cu: operands that the kernels cannot address are copied into a workspace (0 bytes: none is needed); empty sums
+size_t w4_workspace(const W4Args &a);
+int w4_pad_launch(W4Args *a, void *workspace);  // *a then describes the copies
+int w4_zero_launch(const W4Args &a);
 constexpr int kMaxExperts = 4096;
 // qm_w4_rows.cu: few rows of X, mma.sync with weights straight into registers
 bool w4_rows_eligible(const W4Args &a, const DeviceCtx &ctx);
 int w4_rows_launch(const W4Args &a, const DeviceCtx &ctx);
-// qm_w4_tc.cu: tcgen05 with converted weights in TMEM
-bool w4_tc_eligible(const W4Args &a);
+// qm_w4_tc.cu: tcgen05 with converted weights in TMEM; any number of rows of operands that need no copy
 int w4_tc_launch(const W4Args &a, const DeviceCtx &ctx);
 int quantize_w4_launch(const void *W, int type, int64_t ldw, uint8_t *packed, void *scales, int scale_type, int64_t rows, int64_t k, int group,
                        cudaStream_t s);  // qm_w4_quant.cu

@@ -760,12 +760,6 @@ TcPlanW4 tc_plan(const W4Args &a, const DeviceCtx &ctx)
 
 }  // namespace
 
-bool w4_tc_eligible(const W4Args &a)
-{
-    return a.k > 0 && a.k % 32 == 0 && a.ldx % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.B)) & 15u) == 0 &&
-           (int64_t)a.experts * a.n <= 0x7FFFFFFF - 512;
-}
-
 int w4_tc_launch(const W4Args &a, const DeviceCtx &ctx)
 {
     const TcPlanW4 base = tc_plan(a, ctx);

@@ -127,14 +127,23 @@ Weights check_weights(const char *what, const Tensor &x, const Tensor &b, const 
     return w;
 }
 
+// the copies of operands that the kernels cannot address as they are (empty: none are needed)
+Tensor workspace_for(const Tensor &x, const Tensor &b, int64_t experts, const Weights &w)
+{
+    const size_t need = qm_gemm_w4_workspace_bytes(x.data_ptr(), pitch(x), b.data_ptr(), (int)experts, (int)x.size(0), (int)w.n, (int)w.k);
+    return need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+}
+
 Tensor gemm_w4(const Tensor &x, const Tensor &b, const Tensor &scales, int64_t group, const OptTensor &out)
 {
     const char *what = "gemm_w4";
     const Weights w = check_weights(what, x, b, scales, group, false);
     Tensor y = checked_out(what, out, x.size(0), w.n, x);
     c10::cuda::CUDAGuard guard(x.device());
+    const Tensor space = workspace_for(x, b, 1, w);
     check_status(what, qm_gemm_w4(x.data_ptr(), w.type, pitch(x), b.data_ptr(), scales.data_ptr(), w.scale_type, (int)group, y.data_ptr(), pitch(y),
-                                  (int)x.size(0), (int)w.n, (int)w.k, stream_of(x)));
+                                  (int)x.size(0), (int)w.n, (int)w.k, space.defined() ? space.data_ptr() : nullptr,
+                                  space.defined() ? space.numel() : 0, stream_of(x)));
     return y;
 }
 
@@ -148,9 +157,10 @@ Tensor moe_gemm_w4(const Tensor &x, const Tensor &b, const Tensor &scales, const
     if (b.size(0) > INT32_MAX) bad_value(what, "b is too large");
     Tensor y = checked_out(what, out, x.size(0), w.n, x);
     c10::cuda::CUDAGuard guard(x.device());
+    const Tensor space = workspace_for(x, b, b.size(0), w);
     check_status(what, qm_moe_gemm_w4(x.data_ptr(), w.type, pitch(x), b.data_ptr(), scales.data_ptr(), w.scale_type, (int)group,
                                       static_cast<const int *>(offsets.data_ptr()), (int)b.size(0), y.data_ptr(), pitch(y), (int)x.size(0), (int)w.n,
-                                      (int)w.k, stream_of(x)));
+                                      (int)w.k, space.defined() ? space.data_ptr() : nullptr, space.defined() ? space.numel() : 0, stream_of(x)));
     return y;
 }
 

@@ -66,6 +66,16 @@ def pitch(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def _workspace(x, b, experts, n):
+    """(the tensor or None, its pointer, its bytes) for operands that the kernels cannot address as they are."""
+    torch = _torch()
+    need = LIB.qm_gemm_w4_workspace_bytes(x.data_ptr(), pitch(x), b.data_ptr(), experts, x.shape[0], n, x.shape[1])
+    if not need:
+        return None, None, 0
+    space = torch.empty(need, dtype=torch.uint8, device=x.device)
+    return space, space.data_ptr(), need
+
+
 def check_out(what: str, name: str, out, shape, like):
     torch = _torch()
     if out is None:
@@ -104,7 +114,9 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
 
     x: float16 or bfloat16, rows contiguous (a column slab of a wider tensor is fine); b: packed codes [n, k/2] as `pack` and
     `quantize_w4` write them; scales [n, ceil(k / group)]: x's type or float32; group: 32, 64, 128 or 256.  Returns out, of x's
-    type (allocated when not passed in).  Asynchronous on the current stream of x's device."""
+    type (allocated when not passed in).  Sums are fp32; with many rows a weight is rounded to x's type before it is multiplied.
+    k a multiple of 32 and rows of x and b on 16-byte boundaries are fastest: others are copied first.  Asynchronous on the
+    current stream of x's device."""
     what = "gemm_w4"
     if _EXT is not None:
         _count(1)
@@ -113,8 +125,9 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
     m = x.shape[0]
     out = check_out(what, "out", out, (m, n), x)
     with _on_device(x):
-        st = LIB.qm_gemm_w4(x.data_ptr(), code, pitch(x), b.data_ptr(), scales.data_ptr(), scode, group, out.data_ptr(), pitch(out), m, n, k,
-                            _stream_of(x))
+        space, ptr, size = _workspace(x, b, 1, n)
+        st = LIB.qm_gemm_w4(x.data_ptr(), code, pitch(x), b.data_ptr(), scales.data_ptr(), scode, group, out.data_ptr(), pitch(out), m, n, k, ptr,
+                            size, _stream_of(x))
     check(st, f"{what}(m={m}, n={n}, k={k}, group={group})")
     _count(1)
     return out
@@ -141,8 +154,9 @@ def moe_gemm_w4(x, b, scales, offsets, group: int = 128, out=None):
     rows = x.shape[0]
     out = check_out(what, "out", out, (rows, n), x)
     with _on_device(x):
+        space, ptr, size = _workspace(x, b, experts, n)
         st = LIB.qm_moe_gemm_w4(x.data_ptr(), code, pitch(x), b.data_ptr(), scales.data_ptr(), scode, group, offsets.data_ptr(), experts,
-                                out.data_ptr(), pitch(out), rows, n, k, _stream_of(x))
+                                out.data_ptr(), pitch(out), rows, n, k, ptr, size, _stream_of(x))
     check(st, f"{what}(rows={rows}, n={n}, k={k}, experts={experts}, group={group})")
     _count(1)
     return out

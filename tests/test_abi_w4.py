@@ -23,7 +23,7 @@ def p():
 
 def test_gemm_w4(lib, p):
     def call(X=p, type=BF16, ldx=64, B=p, scales=p, scale_type=BF16, group=64, out=p, ldo=8, m=4, n=8, k=64):
-        return lib.qm_gemm_w4(X, type, ldx, B, scales, scale_type, group, out, ldo, m, n, k, None)
+        return lib.qm_gemm_w4(X, type, ldx, B, scales, scale_type, group, out, ldo, m, n, k, None, 0, None)
 
     assert call(m=0) == 0 and call(n=0) == 0 and call(m=0, X=None, out=None) == 0
     assert call(k=63) == SHAPE and call(m=-1) == SHAPE and call(n=-1) == SHAPE and call(k=-2) == SHAPE
@@ -33,12 +33,19 @@ def test_gemm_w4(lib, p):
     for g in (0, -32, 16, 48, 96, 512):
         assert call(group=g) == ARG
     assert call(X=None) == NULL_ and call(B=None) == NULL_ and call(scales=None) == NULL_ and call(out=None) == NULL_
+    # operands off 16-byte boundaries, or k no multiple of 32, need room for copies: rows of k rounded up to 32
+    size = lib.qm_gemm_w4_workspace_bytes
+    assert size(p, 64, p, 1, 4, 8, 64) == 0 and size(p, 64, p, 1, 0, 8, 66) == 0 and size(p, 64, p, 1, 4, 8, 0) == 0
+    assert size(p + 2, 64, p, 1, 4, 8, 64) == size(p, 68, p, 1, 4, 8, 64) == 4 * 64 * 2 and size(p, 64, p + 1, 3, 4, 8, 64) == 3 * 8 * 32
+    assert size(p, 66, p, 1, 4, 8, 66) == 4 * 96 * 2 + 8 * 48
+    assert call(X=p + 2) == WORKSPACE and call(k=62) == WORKSPACE and call(B=p + 1) == WORKSPACE and call(ldx=65) == WORKSPACE
+    assert call(n=2**31 - 512, ldo=2**31) == SHAPE
     assert call(X=p + 1) == ALIGN and call(out=p + 1) == ALIGN and call(scales=p + 1) == ALIGN and call(scales=p + 2, scale_type=F32) == ALIGN
 
 
 def test_moe_gemm_w4(lib, p):
     def call(X=p, offsets=p, experts=2, rows=4, n=8, k=64, group=64, out=p):
-        return lib.qm_moe_gemm_w4(X, BF16, k, p, p, BF16, group, offsets, experts, out, n, rows, n, k, None)
+        return lib.qm_moe_gemm_w4(X, BF16, k, p, p, BF16, group, offsets, experts, out, n, rows, n, k, None, 0, None)
 
     assert call(rows=0) == 0 and call(n=0) == 0 and call(experts=0) == 0
     assert call(offsets=None) == NULL_ and call(offsets=p + 2) == ALIGN and call(experts=-1) == SHAPE and call(rows=-1) == SHAPE
