@@ -20,6 +20,8 @@ def compiled(call, *args):
     try:
         return call(*args)
     except RuntimeError as exc:
+        if type(exc) is not RuntimeError:  # torch's own, such as out of memory
+            raise
         raise QuadmulError(-1, str(exc).split("\n")[0]) from exc
 
 
