@@ -283,7 +283,8 @@ typedef enum qm_type {
  * QM_TYPE_F16 or both QM_TYPE_BF16 (`type`), the scales have that type or QM_TYPE_F32, group is 32, 64, 128 or 256, k is even.
  * Sums are fp32 and are rounded to `type` once; with many rows a weight scale * q is rounded to `type` before it is multiplied
  * (fp16: relative to the largest scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).  A scale
- * that is not finite makes its column not finite.  out is fully overwritten; k == 0 zeroes it.  n * experts is below 2^31 - 512.
+ * that is not finite makes its column not finite; QM_TYPE_BF16 counts scales from 2^126 on among them.  out is fully overwritten;
+ * k == 0 zeroes it.  n * experts is below 2^31 - 512.
  *   k % 32 == 0, ldx % 8 == 0 and 16-byte-aligned X and B need no workspace.  Otherwise X and B are copied into one (device
  *   memory, 16-byte aligned) with k rounded up to 32; qm_gemm_w4_workspace_bytes says how many bytes (experts = 1 for qm_gemm_w4),
  *   QM_ERR_WORKSPACE if there are fewer.

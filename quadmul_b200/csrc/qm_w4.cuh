@@ -70,12 +70,6 @@ int launch_chained(const char *what, void (*kernel)(P...), unsigned blocks, unsi
     return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
 }
 
-inline int launched(const char *what)
-{
-    cudaError_t e = cudaPeekAtLastError();
-    return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
-}
-
 // One lane of the (converged) warp, always the same one.  The code around it stays uniform over the warp, so that the compiler
 // keeps descriptors and addresses in uniform registers, which is where tcgen05.mma and TMA instructions take them: issued from a
 // divergent branch an MMA cost 85 clocks, most of them moves, and 28 from uniform code.
@@ -155,37 +149,19 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, Tag
     return r;
 }
 
-// Eight codes e0 .. e7 of one word -> four pairs (e0, e4), (e1, e5), (e2, e6), (e3, e7) of 16-bit floats, exactly: q for fp16, q / 4
+// Eight codes e0 .. e7 of one word -> four pairs (e0, e1), (e2, e3), (e4, e5), (e6, e7) of 16-bit floats, exactly: q for fp16, q / 4
 // for bf16 (kCodeUnit).  A nibble n is the code q = (n ^ 8) - 8; u = n ^ 8 is made to read as a float and one fma takes the 8 away.
+//   A byte permute puts a byte into both halves of a word; one half keeps the low nibble, the other the high one.
 //   In the last mantissa bits of a power of two whose last place is 1 (bf16 128, fp16 1024) u reads as that power plus u.
 //   fp16 has room for a nibble four bits up, whose last place then counts 1/16.
 //   bf16 has not, but there bits 4 .. 7 with nothing above them are a (sub)normal number u 2^-129: the lowest exponent bit goes
 //   on where the mantissa ends.  fma.bf16x2 keeps subnormal numbers, and 2^127 is the largest factor, hence the quarter.
-// So one shift serves four pairs instead of three.
+// So a pair costs a permute, a lop3 and an fma.
 template <typename T>
 constexpr float kCodeUnit = 1.0f;
 template <>
 constexpr float kCodeUnit<__nv_bfloat16> = 4.0f;
 
-__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
-{
-    const uint32_t w8 = w >> 8;
-    c[0] = fma2(and_xor(w, 0x000F000Fu, 0x43084308u), 0x3E803E80u, 0xC208C208u, tag);   // x 1/4 - 34
-    c[1] = fma2(and_xor(w, 0x00F000F0u, 0x00800080u), 0x7F007F00u, 0xC000C000u, tag);   // x 2^127 - 2
-    c[2] = fma2(and_xor(w8, 0x000F000Fu, 0x43084308u), 0x3E803E80u, 0xC208C208u, tag);
-    c[3] = fma2(and_xor(w8, 0x00F000F0u, 0x00800080u), 0x7F007F00u, 0xC000C000u, tag);
-}
-__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&c)[4], Tag<__half> tag)
-{
-    const uint32_t w8 = w >> 8;
-    c[0] = fma2(and_xor(w, 0x000F000Fu, 0x64086408u), 0x3C003C00u, 0xE408E408u, tag);   // x 1 - 1032
-    c[1] = fma2(and_xor(w, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u, tag);   // x 1/16 - 72
-    c[2] = fma2(and_xor(w8, 0x000F000Fu, 0x64086408u), 0x3C003C00u, 0xE408E408u, tag);
-    c[3] = fma2(and_xor(w8, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u, tag);
-}
-
-// The same eight codes (in the same unit) in their own order: (e0, e1), (e2, e3), (e4, e5), (e6, e7).  A byte permute puts a byte
-// into both halves of a word; one half keeps the low nibble, the other the high one.
 __device__ __forceinline__ void codes_in_order(uint32_t w, uint32_t (&c)[4], Tag<__nv_bfloat16> tag)
 {
 #pragma unroll

@@ -14,10 +14,9 @@
 //
 //  * A CTA (16 warps) takes blocks of 32 rows of B per warp group; WK of its warps split K between them in steps of 128 elements.
 //    Lane (g, q) = (lane / 4, lane % 4) loads 16 bytes, 32 codes, of row g of each 8-row group straight into registers; kDepth steps
-//    are on the way per warp (64 KB per SM; a third costs registers that are not there), across the end of a block, so the
-//    stream does not stop there.  (TMA rings in their
-//    place, one per warp or one per CTA with a loading warp, were slower: a small box costs its thread about 400 clocks, and
-//    1 x 4096 x 4096 has time for four.)
+//    are on the way per warp (64 KB per SM; a third costs registers that are not there), across the end of a block, so the stream
+//    does not stop there.  (TMA rings in their place, one per warp or one per CTA with a loading warp, were slower: a small box
+//    costs its thread about 400 clocks, and 1 x 4096 x 4096 has time for four.)
 //  * A word's even and odd elements are the two halves of an operand fragment; which K an instruction's columns stand for is free
 //    as long as X is laid out alike.  But an instruction adds up over the four lanes of a row, so these must hold codes of
 //    one group: with groups of 128 and more every lane uses its own 32 codes; for 64 and 32 the lanes of a row trade words.

@@ -79,6 +79,28 @@ def test_values_that_are_not_finite_stay_in_their_row(qm, cuda_clean, m):
     assert torch.equal(got[rest], want[rest].to(FP16))
 
 
+@pytest.mark.parametrize("m,group", [(2, 32), (6, 128), (20, 64), (200, 128)])
+@pytest.mark.parametrize("dtype,scale_dtype", [(BF16, BF16), (FP16, FP32)])
+def test_scales_that_are_not_finite_stay_in_their_column(qm, cuda_clean, m, group, dtype, scale_dtype):
+    n, k = 300, 416
+    x, q, packed, scales = whole_case(m, n, k, group, dtype, scale_dtype, 7)
+    scales[5, 1], scales[130, 0], scales[299, -1] = float("inf"), float("nan"), float("-inf")
+    got = run(qm, x, packed, scales, group).cpu()
+    odd = torch.zeros(n, dtype=torch.bool)
+    odd[[5, 130, 299]] = True
+    assert not bool(torch.isfinite(got[:, odd]).any())
+    want = (x.double() @ dequantised(q, scales, group).T).to(dtype)
+    assert torch.equal(got[:, ~odd], want[:, ~odd])
+
+
+@pytest.mark.parametrize("m,n,k,group", [(8, 76000, 640, 128), (5, 20100, 1024, 32), (2, 20011, 2048, 64), (1, 9000, 4096, 256)])
+def test_many_blocks_of_weights(qm, cuda_clean, m, n, k, group):
+    """Few rows and so many of the weights that every warp goes through several blocks of them."""
+    x, q, packed, scales = whole_case(m, n, k, group, BF16, BF16, 11)
+    want = (x.double() @ dequantised(q, scales, group).T).to(BF16)
+    assert torch.equal(run(qm, x, packed, scales, group).cpu(), want)
+
+
 @pytest.mark.parametrize("m", [2, 20, 200])
 @pytest.mark.parametrize("size,x_size", [(2.0**-20, 2.0**13), (2.0**-3, 1.0), (2.0**14, 2.0**-12)])
 def test_fp16_with_small_and_large_scales(qm, cuda_clean, m, size, x_size):
@@ -186,6 +208,18 @@ def test_experts(qm, cuda_clean, offsets, n, k, group, dtype, scale_dtype):
     x, q, packed, scales = whole_case(rows, n, k, group, dtype, scale_dtype, 20, (experts,))
     x[offsets[-1] :] = float("nan")  # what no expert has is not read into any result
     out = torch.full((rows, n), SENTINEL, dtype=dtype)
+    got = qm.moe_gemm_w4(x.cuda(), packed.cuda(), scales.cuda(), torch.tensor(offsets, dtype=torch.int32).cuda(), group, out=out.cuda())
+    assert torch.equal(got.cpu(), expert_reference(x, q, scales, group, offsets, out))
+
+
+@pytest.mark.parametrize("n,k,rows,longest", [(200, 320, 190, 150), (3300, 128, 190, 100), (130, 256, 1000, 700)])
+def test_one_long_segment_among_short_ones(qm, cuda_clean, n, k, rows, longest):
+    experts, group = 24, 64
+    x, q, packed, scales = whole_case(rows, n, k, group, BF16, BF16, 24, (experts,))
+    before = sorted(torch.randint(0, rows - longest + 1, (experts // 2,), generator=torch.Generator().manual_seed(4)).tolist())
+    after = sorted(torch.randint(before[-1] + longest, rows + 1, (experts // 2,), generator=torch.Generator().manual_seed(5)).tolist())
+    offsets = before + after + [rows]
+    out = torch.full((rows, n), SENTINEL, dtype=BF16)
     got = qm.moe_gemm_w4(x.cuda(), packed.cuda(), scales.cuda(), torch.tensor(offsets, dtype=torch.int32).cuda(), group, out=out.cuda())
     assert torch.equal(got.cpu(), expert_reference(x, q, scales, group, offsets, out))
 
