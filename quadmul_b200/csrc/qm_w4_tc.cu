@@ -447,8 +447,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                 const uint32_t src = w0 + ws * kBytesW + (uint32_t)r * 64;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = lds128(src + (((uint32_t)j ^ swz) << 4));
-                __syncwarp();
-                if (lane == 0) mbar_arrive(w_empty(ws));  // the codes are in registers
                 if (!warp_wait<false>(ax_empty(s), ((i / kRingX) & 1u) ^ 1u, abort_flag, lane)) {
                     if (lane == 0) give_up(kWaitConvertSlot);
                     ok = false;
@@ -486,6 +484,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
+                    // The codes' slot is handed back only here, where they have been used.  Handed back behind the loads, with the
+                    // wait for the stage in between, it was filled again before they had returned: an arrive does not wait for
+                    // loads on their way, and the next copy comes through another proxy.
+                    mbar_arrive(w_empty(ws));
                     if constexpr (G == 2) mbar_arrive_cluster(a_full(s), 0);
                     else mbar_arrive(a_full(s));
                 }

@@ -180,6 +180,67 @@ def test_equal_calls_give_equal_bits(qm, cuda_clean):
             assert torch.equal(first, qm.gemm_w4(*args))
 
 
+@pytest.mark.parametrize("m,n,k,group", [(17, 20070, 4096, 128), (64, 40000, 1024, 64), (96, 20070, 4096, 128), (200, 20070, 2048, 32), (500, 19000, 1024, 128)])
+@pytest.mark.parametrize("dtype,scale_dtype", [(BF16, BF16), (FP16, FP32)])
+def test_many_tiles_of_many_steps(qm, cuda_clean, m, n, k, group, dtype, scale_dtype):
+    """Every pair of SMs goes through several tiles, a few dozen steps each, and the rings between its warps wrap at any place."""
+    gen = torch.Generator().manual_seed(14)
+    x = torch.randint(-1, 2, (m, k), generator=gen).to(dtype)
+    q, packed = codes((n, k), gen)
+    scales = torch.exp2(torch.randint(-2, 2, (n, k // group), generator=gen).double()).to(scale_dtype)
+    w = dequantised(q, scales, group).float()  # exact, as is the product: multiples of 1/4 below 2^19
+    want = (x.float() @ w.T).to(dtype)
+    args = (x.cuda(), packed.cuda(), scales.cuda(), group)
+    for _ in range(5):
+        assert torch.equal(qm.gemm_w4(*args).cpu(), want)
+
+
+def test_many_tiles_of_experts(qm, cuda_clean):
+    experts, n, k, group = 24, 2000, 1024, 128
+    offsets = torch.cumsum(torch.randint(5, 70, (experts + 1,), generator=torch.Generator().manual_seed(3)), 0).int()
+    rows = int(offsets[-1])
+    x, q, packed, scales = whole_case(rows, n, k, group, BF16, BF16, 15, (experts,))
+    args = (x.cuda(), packed.cuda(), scales.cuda(), offsets.cuda(), group)
+    out = torch.full((rows, n), SENTINEL, dtype=BF16)
+    want = expert_reference(x, q, scales, group, offsets.tolist(), out)
+    for _ in range(5):
+        assert torch.equal(qm.moe_gemm_w4(*args, out=out.cuda()).cpu(), want)
+
+
+@pytest.mark.parametrize("m", [2, 40])
+def test_weights_of_more_than_32_bits(qm, cuda_clean, m):
+    """The packed matrix has more than 2^32 bytes, the output of the next test more than 2^31 elements."""
+    n, k, group = (1 << 20) + 70, 8192 + 32, 128
+    b = torch.randint(-128, 128, (n, k // 2), dtype=torch.int8, device="cuda")
+    scales = torch.exp2(torch.randint(-2, 2, (n, -(-k // group)), device="cuda").float()).to(BF16)
+    x = torch.randint(-1, 2, (m, k), generator=torch.Generator().manual_seed(1)).to(BF16)
+    got = qm.gemm_w4(x.cuda(), b, scales, group)
+    for first in (0, n // 2, n - 200):
+        part = slice(first, first + 200)
+        w = dequantised(qm.unpack(b[part].contiguous()).cpu(), scales[part].cpu(), group)
+        assert torch.equal(got[:, part].cpu(), (x.double() @ w.T).to(BF16))
+
+
+def test_output_of_more_than_32_bits(qm, cuda_clean):
+    rows, n, k, group = 600_000, 4096, 64, 32
+    _, q, packed, scales = whole_case(1, n, k, group, BF16, BF16, 13, (2,))
+    x = torch.randint(-3, 4, (rows, k), generator=torch.Generator().manual_seed(2)).to(BF16)
+    offsets = torch.tensor([0, 100, rows], dtype=torch.int32, device="cuda")
+    got = qm.moe_gemm_w4(x.cuda(), packed.cuda(), scales.cuda(), offsets, group)
+    for first, e in ((0, 0), (rows // 2, 1), (rows - 100, 1)):
+        part = slice(first, first + 100)
+        assert torch.equal(got[part].cpu(), (x[part].double() @ dequantised(q[e], scales[e], group).T).to(BF16))
+    weights = torch.ones(rows // 2, 2, dtype=BF16, device="cuda")
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda").view(-1, 2)
+    y = qm.moe_combine(got, slots, weights)
+    assert torch.equal(y[-5:], (got[-10::2].float() + got[-9::2].float()).to(BF16))
+    dys, dw = qm.moe_combine_grad(y, got, slots, weights)
+    assert torch.equal(dys[-10::2], y[-5:]) and torch.equal(dys[-9::2], y[-5:])
+    ids = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    xs, _, slots = qm.moe_sort(got, ids, 1, out=dys)
+    assert torch.equal(xs[-5:], got[-5:]) and slots[-1, 0] == rows - 1
+
+
 # ---- experts ---------------------------------------------------------------------------------------------------------------
 
 
