@@ -357,7 +357,7 @@ int moe_sort_launch(const MoeSortArgs &a)
     auto by_id = [&](auto id) {
         using I = typename decltype(id)::type;
         const I *ids = static_cast<const I *>(a.ids);
-        if (count > kFewIds) {
+        if (count > kFewIds && a.experts > 0) {  // (without experts there is nothing to count)
             totals = a.workspace;
             counts = a.workspace + a.experts;
             int st = launch_chained("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kSortThreads, (size_t)a.experts * sizeof(int), a.stream, ids,

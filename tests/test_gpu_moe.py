@@ -189,6 +189,12 @@ def test_empty_sizes(qm, cuda_clean):
     assert bool((qm.moe_combine(xs, slots) == 0).all())
     xs, offsets, slots = qm.moe_sort(x, torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 0)
     assert offsets.tolist() == [0] and slots.flatten().tolist() == [-1] * 6
+    many = torch.ones(9000, 8, device="cuda")  # more ids than one launch sorts
+    _, offsets, slots = qm.moe_sort(many, torch.zeros(9000, 2, dtype=torch.int32, device="cuda"), 0)
+    assert offsets.tolist() == [0] and bool((slots == -1).all())
+    y = qm.moe_linear_w4(many.bfloat16(), torch.zeros(9000, 2, dtype=torch.int32, device="cuda"), torch.ones(9000, 2, device="cuda"),
+                         torch.zeros(0, 6, 4, dtype=torch.int8, device="cuda"), torch.zeros(0, 6, 1, dtype=BF16, device="cuda"))
+    assert y.shape == (9000, 6) and bool((y == 0).all())
     xs, offsets, slots = qm.moe_sort(x[:, :0], torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 2)
     assert xs.shape == (6, 0) and offsets.tolist() == [0, 6, 6] and slots.flatten().tolist() == list(range(6))
     dys, dw = qm.moe_combine_grad(x[:, :0], xs, slots, torch.ones(3, 2, device="cuda"))
