@@ -284,7 +284,7 @@ typedef enum qm_type {
  * Sums are fp32 and are rounded to `type` once; with many rows a weight scale * q is rounded to `type` before it is multiplied
  * (fp16: relative to the largest scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).  A scale
  * that is not finite makes its column not finite; QM_TYPE_BF16 counts scales from 2^126 on among them.  out is fully overwritten;
- * k == 0 zeroes it.  n * experts is below 2^31 - 512.
+ * k == 0 zeroes it, k is at most 2^30 - 32.  n * experts is below 2^31 - 512.  out shares no element with the inputs, here and below.
  *   k % 32 == 0, ldx % 8 == 0 and 16-byte-aligned X and B need no workspace.  Otherwise X and B are copied into one (device
  *   memory, 16-byte aligned) with k rounded up to 32; qm_gemm_w4_workspace_bytes says how many bytes (experts = 1 for qm_gemm_w4),
  *   QM_ERR_WORKSPACE if there are fewer.
@@ -340,7 +340,8 @@ int qm_moe_combine(const void *ys, int type, int64_t ldys, int rows, const int *
 
 /*
  * The gradients of qm_moe_combine: dys[slots[t][j]] = weights[t][j] * dy[t] (rows that no slot names are left as they were) and
- * dweights[t][j] = <dy[t], ys[slots[t][j]]> in fp32, rounded to weight_type (0 for a slot outside [0, rows)).
+ * dweights[t][j] = <dy[t], ys[slots[t][j]]> in fp32, rounded to weight_type (0 for a slot outside [0, rows)).  Slots within
+ * [0, rows) differ from one another, as those of qm_moe_sort do.
  */
 int qm_moe_combine_grad(const void *dy, int64_t lddy, const void *ys, int64_t ldys, int type, int rows, const int *slots,
                         const void *weights, int weight_type, void *dys, int64_t lddys, void *dweights, int tokens, int top_k,

@@ -8,13 +8,15 @@ using namespace qm;
 
 namespace {
 
+constexpr int kMaxK = (1 << 30) - 32;  // a row of X is below 2^31 bytes, rounded up to 32 elements or not
+
 bool known_group(int g) { return g == 32 || g == 64 || g == 128 || g == 256; }
 
 bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 int check_w4(const W4Args &a)
 {
-    if (a.rows < 0 || a.n < 0 || a.k < 0 || (a.k & 1) || a.experts < 0 || a.experts > kMaxExperts) return QM_ERR_SHAPE;
+    if (a.rows < 0 || a.n < 0 || a.k < 0 || (a.k & 1) || a.k > kMaxK || a.experts < 0 || a.experts > kMaxExperts) return QM_ERR_SHAPE;
     if (a.type != QM_TYPE_F16 && a.type != QM_TYPE_BF16) return QM_ERR_ARG;
     if (a.scale_type != QM_TYPE_F32 && a.scale_type != a.type) return QM_ERR_ARG;
     if (!known_group(a.group)) return QM_ERR_ARG;

@@ -5,7 +5,8 @@
   moe_sort_grad, moe_combine_grad      their gradients, as calls of their own (nothing here is recorded by autograd)
   moe_linear_w4(...)                   the three steps of one 4-bit expert projection
 
-The reference has no counterpart.  Everything is deterministic: there are no floating-point atomics.
+The reference has no counterpart.  Everything is deterministic: there are no floating-point atomics.  An `out` must not share
+elements with the inputs.
 """
 from __future__ import annotations
 

@@ -5,7 +5,8 @@
   moe_gemm_w4(x, b, ...)      the same with one matrix per expert over rows sorted by expert (moe.moe_sort)
 
 The reference has no counterpart: its only product is s4 x s4.  Sums are fp32.  The packed weights carry no gradient, and the
-products are not recorded by autograd: an input that requires a gradient is refused while gradients are enabled.
+products are not recorded by autograd: an input that requires a gradient is refused while gradients are enabled.  An `out` must
+not share elements with the inputs.
 """
 from __future__ import annotations
 
@@ -167,9 +168,9 @@ def moe_gemm_w4(x, b, scales, offsets, group: int = 128, out=None):
 def quantize_w4(w, group: int = 128, scale_dtype=None):
     """w [n, k] (float32, float16 or bfloat16) -> (packed codes [n, k/2] int8, scales [n, ceil(k / group)]).
 
-    Per group of a row: scale = max |w| times the float32 value of 1/7, rounded to scale_dtype (w's type by default, or float32); code = w / scale rounded to
-    the nearest integer, ties to even, within [-8, 7].  A group of zeros has scale 0; a group that holds an infinity or a NaN
-    has a scale that is not finite and codes 0."""
+    Per group of a row: scale = max |w| times the float32 value of 1/7, rounded to scale_dtype (w's type by default, or float32);
+    code = w / scale rounded to the nearest integer, ties to even, within [-8, 7].  A group of zeros has scale 0; a group that
+    holds an infinity or a NaN has a scale that is not finite and codes 0."""
     what = "quantize_w4"
     torch = _torch()
     scale_dtype = w.dtype if scale_dtype is None else scale_dtype

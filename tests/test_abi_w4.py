@@ -40,6 +40,7 @@ def test_gemm_w4(lib, p):
     assert size(p, 66, p, 1, 4, 8, 66) == 4 * 96 * 2 + 8 * 48
     assert call(X=p + 2) == WORKSPACE and call(k=62) == WORKSPACE and call(B=p + 1) == WORKSPACE and call(ldx=65) == WORKSPACE
     assert call(n=2**31 - 512, ldo=2**31) == SHAPE
+    assert call(k=2**30 - 30, ldx=2**30) == SHAPE and call(k=2**30 - 30, ldx=2**30, m=0) == SHAPE and call(k=2**31 - 2, ldx=2**31) == SHAPE
     assert call(X=p + 1) == ALIGN and call(out=p + 1) == ALIGN and call(scales=p + 1) == ALIGN and call(scales=p + 2, scale_type=F32) == ALIGN
 
 
