@@ -53,6 +53,7 @@ constexpr int kAccCols = 256, kStageCols = 64, kTmemCols = 512;
 constexpr int kEpiWarp = 4, kNumEpiWarps = 8, kConvWarp = 12, kSets = 3, kNumConvWarps = 4 * kSets;
 constexpr int kNumWarps = kConvWarp + kNumConvWarps, kNumThreads = kNumWarps * 32;
 constexpr int kNumBarriers = 2 * kRingW + 3 * kRingX + 2;
+constexpr int kMaxParts = 8;    // of K: a cluster
 constexpr int kEpiBytes = 16 * 32 * 2;  // per epilogue warp: 16 rows of out x 32 columns
 constexpr int kSmemFixed = 1024 + kRingW * kBytesW + kRingX * kBytesX + kNumEpiWarps * kEpiBytes + kNumBarriers * 8 + 16 + kRowsB * 4;
 static_assert(kAccCols + kRingX * kStageCols <= kTmemCols, "TMEM budget");
@@ -147,29 +148,43 @@ __device__ __forceinline__ float row_unit(const S *__restrict__ s, int groups)
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         return 1.0f;
     } else {
-        float top = 0.0f;
-        bool nan = false;
-        int j = 0;
-        constexpr int kVec = 16 / (int)sizeof(S);
-        if ((reinterpret_cast<uintptr_t>(s) & 15u) == 0) {
-            for (; j + kVec <= groups; j += kVec) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(s + j));
-                const S *e = reinterpret_cast<const S *>(&v);
+        // Magnitudes order like unsigned integers, an infinity or a NaN above every number.  The loads go out many at a time: the
+        // row comes from DRAM, and a few in turn held 37 x 1100 x 2208 up for 9,000 clocks.  (Those behind the end repeat the last.)
+        uint32_t most = 0;
+        constexpr int kVec = 16 / (int)sizeof(S), kAhead = 4;
+        if ((reinterpret_cast<uintptr_t>(s) & 15u) == 0 && groups % kVec == 0) {
+            const uint4 *v = reinterpret_cast<const uint4 *>(s);
+            const int last = groups / kVec - 1;
+            for (int j = 0; j <= last; j += kAhead) {
+                uint4 u[kAhead];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float f = to_float(e[i]);
-                    nan |= f != f;
-                    top = fmaxf(top, fabsf(f));
+                for (int i = 0; i < kAhead; ++i) u[i] = __ldg(v + min(j + i, last));
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) {
+                        if constexpr (sizeof(S) == 4) most = max(most, w[o] & 0x7FFFFFFFu);
+                        else most = __vmaxu2(most, w[o] & 0x7FFF7FFFu);
+                    }
                 }
             }
+            if constexpr (sizeof(S) == 2) most = max(most & 0xFFFFu, most >> 16);
+        } else {
+            using Bits = typename std::conditional<sizeof(S) == 4, uint32_t, unsigned short>::type;
+            const Bits *v = reinterpret_cast<const Bits *>(s);
+            for (int j = 0; j < groups; j += 4 * kAhead) {
+                uint32_t u[4 * kAhead];
+#pragma unroll
+                for (int i = 0; i < 4 * kAhead; ++i) u[i] = __ldg(v + min(j + i, groups - 1));
+#pragma unroll
+                for (int i = 0; i < 4 * kAhead; ++i) most = max(most, u[i] & (sizeof(S) == 4 ? 0x7FFFFFFFu : 0x7FFFu));
+            }
         }
-#pragma unroll 4
-        for (; j < groups; ++j) {
-            const float f = to_float(s[j]);
-            nan |= f != f;
-            top = fmaxf(top, fabsf(f));
-        }
-        if (nan || !(top > 0.0f) || top == INFINITY) return 1.0f;
+        float top;
+        if constexpr (sizeof(S) == 4) top = __uint_as_float(most);
+        else top = __half2float(__ushort_as_half((unsigned short)most));
+        if (!(top > 0.0f) || !(top < INFINITY)) return 1.0f;
         // exponent bits alone; the smallest normal number for a subnormal one, and no larger than leaves a finite reciprocal
         const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
         return __uint_as_float(e << 23);
@@ -229,8 +244,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
     if (p.offsets && warp == 3) scan_segments(p.offsets, p.experts, p.rows, p.tile, seg, tiles, lane);
     tc_fence_before_sync();
     __syncthreads();
-    cluster_arrive();
-    cluster_wait();
+    if (G == 2) {  // the pair's barriers are there (in the SPLIT form a CTA keeps to itself until the parts are added up)
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
     const uint32_t tmem_a0 = tmem_base + kAccCols;
@@ -589,11 +606,14 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
                 for (int i = threadIdx.x; i < todo * (kRowsB / 2); i += kNumThreads) {
                     const int row = rank + (i / (kRowsB / 2)) * parts, pos = (i % (kRowsB / 2)) * 2, col = m.col + pos;
                     if (col >= p.n) continue;
+                    float2 v[kMaxParts];
+#pragma unroll
+                    for (int o = 0; o < kMaxParts; ++o)
+                        if (o < parts) v[o] = lds_cluster_f2(mapa_cluster(x0 + (uint32_t)(row * kRowsB + pos) * 4u, (uint32_t)o));
                     float a = 0.0f, b = 0.0f;
-                    for (int o = 0; o < parts; ++o) {
-                        const float2 v = lds_cluster_f2(mapa_cluster(x0 + (uint32_t)(row * kRowsB + pos) * 4u, (uint32_t)o));
-                        a += v.x, b += v.y;
-                    }
+#pragma unroll
+                    for (int o = 0; o < kMaxParts; ++o)
+                        if (o < parts) a += v[o].x, b += v[o].y;
                     const uint32_t two = pack2(a * unit_of_row[pos], b * unit_of_row[pos + 1], Tag<T>());
                     unsigned short *dst = reinterpret_cast<unsigned short *>(out + (int64_t)(m.row + row) * p.ldo + col);
                     if (p.vec_out && col + 1 < p.n) {
@@ -742,7 +762,7 @@ TcPlanW4 tc_plan(const W4Args &a, const DeviceCtx &ctx)
         plan.pair = 0;
         plan.tile = 128;
         int parts = (int)(ctx.num_sms / single);
-        if (parts > 8) parts = 8;
+        if (parts > kMaxParts) parts = kMaxParts;
         if (parts > num_kb) parts = num_kb;
         plan.parts = parts < 1 ? 1 : parts;
         return plan;
