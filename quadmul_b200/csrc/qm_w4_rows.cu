@@ -46,7 +46,7 @@ constexpr int kDepth = 2;                          // steps on the way per warp
 constexpr int kStep = 128;                         // elements of K per step
 constexpr int kRG = 4, kTiles = 2, kRows = 8 * kRG;  // 8-row groups, 16-row tiles and rows of B per warp
 constexpr int kRedFloats = kWarps * kTiles * 128;  // one of two buffers
-constexpr int kMaxSmem = 232448 - 1024;
+constexpr int kMaxSmem = 232448;  // eight rows of 8192 elements just fit
 constexpr int kNarrowRows = 2, kWideRows = 8;
 
 struct RowsParams {

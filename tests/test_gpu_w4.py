@@ -15,7 +15,8 @@ SHAPES = [
     (9, 129, 256, 128), (15, 16, 4096, 128), (16, 257, 2208, 64), (17, 32, 1056, 32), (31, 100, 64, 256), (32, 256, 512, 64), (33, 1100, 2208, 64),
     (63, 65, 96, 32), (64, 128, 4128, 128), (65, 300, 1024, 256), (100, 40, 6, 32), (127, 127, 1022, 64), (128, 256, 256, 128), (129, 200, 320, 64),
     (255, 257, 512, 32), (256, 256, 384, 128), (257, 520, 64, 64), (300, 130, 4064, 256), (513, 384, 1024, 128), (1, 4096, 4096, 128),
-    (4, 1024, 11008, 128), (16, 512, 11008, 64), (600, 72, 94, 128),
+    (4, 1024, 11008, 128), (16, 512, 11008, 64), (600, 72, 94, 128), (8, 300, 8192, 128), (8, 5000, 8192, 256), (3, 300, 8192, 64), (2, 300, 16384, 128),
+    (1, 100, 30000, 32), (2, 64, 65536, 128),
 ]
 
 
