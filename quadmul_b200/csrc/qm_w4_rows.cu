@@ -26,6 +26,10 @@
 //    Otherwise (1 or 2 rows) the three bytes of both rows take six columns of one instruction.
 //  * The warps' partial tiles meet in shared memory (two buffers, one barrier a block) and are added in a fixed order.
 //
+// Measured (groups of 128, bf16): 1 x 57344 x 8192 54 us = 4.45 TB/s, 8 rows of it 87 us; 1 x 4096 x 4096 5.2 us, of which a launch
+// in a dependent chain is 2.4; 128 rows over 32 experts of 4096 x 4096 72 us = 3.9 TB/s, DRAM at 47 % and the s8 pipe at 36 % of
+// their peaks.  Groups of 32 cost 1.3 us more at 1 x 4096 x 4096: the lanes trade words.
+//
 // With experts a unit of work is (expert, tile of its rows, block of B); every CTA takes a contiguous range of units, so the rows
 // of X change rarely.
 #include <atomic>
