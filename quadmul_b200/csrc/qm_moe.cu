@@ -8,10 +8,12 @@
 // the counts over the blocks, and the placing.  With up to 64 experts ids are counted without atomics: a lane has the counts of
 // one or two experts in registers, and finds who of 32 ids names them from a ballot per bit of the id.
 //
-// Measured (bf16): sort of 16 x 8 by 64 experts 5.5 us, of 8192 x 2 rows of 4096 45 us = 4.5 TB/s; combine of 4096 x 8 rows of
+// The launches take their turn in the stream: these kernels read indices that the kernel before may have written, and addresses come
+// from them, so none starts before that one has ended.
+//
+// Measured (bf16): sort of 16 x 8 by 64 experts 5.9 us, of 8192 x 2 rows of 4096 45 us = 4.5 TB/s; combine of 4096 x 8 rows of
 // 4096 47 us = 6.4 TB/s, its gradients 90 us = 6.4 TB/s (0.97 of a copy).  Single elements (rows off 16-byte boundaries, 3000 x 4 of
 // 5119): sort 66 us = 2.3 TB/s, combine 49 us = 3.1.
-#include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
 namespace qm {
@@ -87,8 +89,6 @@ template <typename I>
 __global__ void __launch_bounds__(kSortThreads) moe_count_kernel(const I *__restrict__ ids, int experts, int count, int per_block, int *__restrict__ counts)
 {
     extern __shared__ int mine[];
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     for (int e = threadIdx.x; e < experts; e += kSortThreads) mine[e] = 0;
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * per_block;
@@ -100,8 +100,6 @@ __global__ void __launch_bounds__(kSortThreads) moe_count_kernel(const I *__rest
 // counts[block][expert] -> how many earlier blocks have, totals[expert]; one warp per expert
 __global__ void __launch_bounds__(kThreads) moe_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int experts, int blocks)
 {
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     const int e = (int)(blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
     if (e >= experts) return;
     int sum = 0;
@@ -130,8 +128,6 @@ __global__ void __launch_bounds__(kSortThreads) moe_place_kernel(const T *__rest
     extern __shared__ int smem[];
     int *next = smem, *total = smem + experts, *at = total + experts;  // at: the experts, then the slots of the block's assignments
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     const int64_t first = (int64_t)blockIdx.x * per_block * top_k;
     const int64_t last = min((int64_t)tokens * top_k, first + (int64_t)per_block * top_k);
     for (int e = threadIdx.x; e < experts; e += kSortThreads) {
@@ -217,8 +213,6 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
                                                                const S *__restrict__ weights, T *__restrict__ y, int64_t ldy, int top_k, int hidden,
                                                                int parts)
 {
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     constexpr int kAhead = 8;                // rows in flight per thread
     constexpr int kCols = VEC == 1 ? 4 : 1;  // pieces of a row per thread and turn: single elements need more of them in flight
     const int64_t t = blockIdx.x / parts;
@@ -272,8 +266,6 @@ __global__ void __launch_bounds__(kThreads) moe_combine_grad_kernel(const T *__r
                                                                     const int *__restrict__ slots, const S *__restrict__ weights, T *__restrict__ dys,
                                                                     int64_t lddys, S *__restrict__ dweights, int top_k, int hidden)
 {
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     constexpr int kAhead = 4;
     __shared__ float part[kThreads / 32][kAhead];
     const int64_t t = blockIdx.x;
@@ -364,10 +356,10 @@ int moe_sort_launch(const MoeSortArgs &a)
         if (count > kFewIds && a.experts > 0) {  // (without experts there is nothing to count)
             totals = a.workspace;
             counts = a.workspace + a.experts;
-            int st = launch_chained("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kSortThreads, (size_t)a.experts * sizeof(int), a.stream, ids,
+            int st = launch_in_turn("moe_count_kernel launch", moe_count_kernel<I>, (unsigned)blocks, kSortThreads, (size_t)a.experts * sizeof(int), a.stream, ids,
                                     a.experts, count, per * a.top_k, counts);
             if (st != QM_OK) return st;
-            st = launch_chained("moe_scan_kernel launch", moe_scan_kernel, (unsigned)((a.experts + 7) / 8), kThreads, 0, a.stream, counts, totals, a.experts,
+            st = launch_in_turn("moe_scan_kernel launch", moe_scan_kernel, (unsigned)((a.experts + 7) / 8), kThreads, 0, a.stream, counts, totals, a.experts,
                                 blocks);
             if (st != QM_OK) return st;
         }
@@ -381,7 +373,7 @@ int moe_sort_launch(const MoeSortArgs &a)
                     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
                     if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(moe_place_kernel)");
                 }
-                return launch_chained("moe_place_kernel launch", kernel, (unsigned)blocks, kSortThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
+                return launch_in_turn("moe_place_kernel launch", kernel, (unsigned)blocks, kSortThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
                                       a.experts, a.tokens, a.top_k, a.hidden, per, (const int *)counts, (const int *)totals, static_cast<T *>(a.xs), a.ldxs,
                                       a.offsets, a.slots);
             });
@@ -403,7 +395,7 @@ int moe_combine_launch(const MoeCombineArgs &a)
                 constexpr int kStretch = kThreads * (VEC == 1 ? 4 : VEC);
                 int64_t parts = (a.hidden + kStretch - 1) / kStretch;
                 if (parts * a.tokens > 0x7FFFFFFF) parts = 1;
-                return launch_chained("moe_combine_kernel launch", moe_combine_kernel<T, S, VEC>, (unsigned)(parts * a.tokens), kThreads, 0, a.stream,
+                return launch_in_turn("moe_combine_kernel launch", moe_combine_kernel<T, S, VEC>, (unsigned)(parts * a.tokens), kThreads, 0, a.stream,
                                       static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots, static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo,
                                       a.top_k, a.hidden, (int)parts);
             });
@@ -421,7 +413,7 @@ int moe_combine_grad_launch(const MoeCombineArgs &a)
                              a.hidden % (16 / (int)sizeof(T)) == 0;
             return with_pieces<T>(vec, [&](auto v) {
                 constexpr int VEC = decltype(v)::value;
-                return launch_chained("moe_combine_grad_kernel launch", moe_combine_grad_kernel<T, S, VEC>, (unsigned)a.tokens, kThreads, 0, a.stream,
+                return launch_in_turn("moe_combine_grad_kernel launch", moe_combine_grad_kernel<T, S, VEC>, (unsigned)a.tokens, kThreads, 0, a.stream,
                                       static_cast<const T *>(a.dy), a.lddy, static_cast<const T *>(a.ys), a.ldys, a.rows, a.slots,
                                       static_cast<const S *>(a.weights), static_cast<T *>(a.out), a.ldo, static_cast<S *>(a.dweights), a.top_k, a.hidden);
             });

@@ -70,6 +70,19 @@ int launch_chained(const char *what, void (*kernel)(P...), unsigned blocks, unsi
     return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
 }
 
+// Launch behind everything the stream has before it.
+template <typename... P, typename... A>
+int launch_in_turn(const char *what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? QM_OK : record_cuda_error(e, what);
+}
+
 // One lane of the (converged) warp, always the same one.  The code around it stays uniform over the warp, so that the compiler
 // keeps descriptors and addresses in uniform registers, which is where tcgen05.mma and TMA instructions take them: issued from a
 // divergent branch an MMA cost 85 clocks, most of them moves, and 28 from uniform code.

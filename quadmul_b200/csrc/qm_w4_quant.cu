@@ -9,7 +9,6 @@
 // 3.4 TB/s, bound by the arithmetic.  Any alignment: 11008 x 4094 bf16 108 us.
 #include <type_traits>
 
-#include "qm_ptx.cuh"
 #include "qm_w4.cuh"
 
 namespace qm {
@@ -150,8 +149,6 @@ template <typename T, typename S>
 __global__ void __launch_bounds__(kThreads, 4) quantize_w4_kernel(const T *__restrict__ W, int64_t ldw, uint8_t *__restrict__ packed, S *__restrict__ scales,
                                                                int rows, int k, int group_shift)
 {
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int lanes = 1 << (group_shift - 4);  // lanes that share a group
     const int per_row = (k + 511) / 512, groups = (k + (1 << group_shift) - 1) >> group_shift;
@@ -196,8 +193,6 @@ template <typename T, typename S>
 __global__ void __launch_bounds__(kThreads) quantize_w4_any_kernel(const T *__restrict__ W, int64_t ldw, uint8_t *__restrict__ packed,
                                                                    S *__restrict__ scales, int64_t rows, int64_t k, int group)
 {
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int64_t groups = (k + group - 1) / group, all = rows * groups;
     for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < all; i += (int64_t)gridDim.x * (kThreads / 32)) {
@@ -248,11 +243,11 @@ int quantize_w4_launch(const void *W, int type, int64_t ldw, uint8_t *packed, vo
                              (ldw * (int64_t)sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(packed) & 7u) == 0;
             if (vec) {
                 const int64_t pieces = rows * ((k + 511) / 512), blocks = (pieces + 8 * kUnroll - 1) / (8 * kUnroll);
-                return launch_chained("quantize_w4_kernel launch", quantize_w4_kernel<T, S>, (unsigned)(blocks < 148 * 4 ? blocks : 148 * 4), kThreads, 0,
+                return launch_in_turn("quantize_w4_kernel launch", quantize_w4_kernel<T, S>, (unsigned)(blocks < 148 * 4 ? blocks : 148 * 4), kThreads, 0,
                                       stream, w, ldw, packed, s, (int)rows, (int)k, group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8);
             }
             const int64_t blocks = (rows * ((k + group - 1) / group) + 7) / 8;
-            return launch_chained("quantize_w4_any_kernel launch", quantize_w4_any_kernel<T, S>, (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), kThreads,
+            return launch_in_turn("quantize_w4_any_kernel launch", quantize_w4_any_kernel<T, S>, (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), kThreads,
                                   0, stream, w, ldw, packed, s, rows, k, group);
         });
     });
