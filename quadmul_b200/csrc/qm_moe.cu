@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kSortThreads) moe_place_kernel(const T *__rest
             const int e = i < (int)(last - first) ? at[i] : -1;
             const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
             const int rank = __popc(same & ((1u << lane) - 1u));
-            const int slot = e >= 0 ? next[e] + rank : -1;
+            // (a slot is below all assignments unless the ids were changed under way: nothing is written outside xs then either)
+            const int place = e >= 0 ? next[e] + rank : -1, slot = place < tokens * top_k ? place : -1;
             __syncwarp();
             if (e >= 0 && rank == 0) next[e] += __popc(same);
             __syncwarp();
