@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kNumThreads, R)
 gemm_dec_kernel(const __grid_constant__ CUtensorMap tmapP, const __grid_constant__ CUtensorMap tmapQ,
                 int32_t *__restrict__ C, int64_t ldc, int rowsP, int rowsQ, int K, int *status, int split_k, int parts_stride,
                 int32_t *__restrict__ scratch, int *__restrict__ counters, uint16_t *__restrict__ out_bf16,
-                const float *__restrict__ scale_a, const float *__restrict__ scale_b)
+                const float *scale_a, const float *scale_b)
 {
     // out_bf16 != NULL: fused dequantisation, out[q][p] = bf16(float(sum) * scale_a[q] * scale_b[p]) instead of C[q][p] = sum
     // (q = row of A, p = row of B; a NULL scale vector is all ones).
@@ -380,12 +380,12 @@ gemm_dec_kernel(const __grid_constant__ CUtensorMap tmapP, const __grid_constant
                 constexpr int SHIFT = decltype(shift_tag)::value;
                 if (p >= rowsP) return;
                 if (out_bf16) {
-                    const float sbp = scale_b ? __ldg(scale_b + p) : 1.0f;
+                    const float sbp = scale_b ? ld_behind_wait(scale_b + p) : 1.0f;
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (q_first + j < rowsQ)
                             out_bf16[(int64_t)(q_first + j) * ldc + p] = (uint16_t)dequant_bf16_bits(
-                                (int32_t)vals[first + j] >> SHIFT, scale_a ? __ldg(scale_a + q_first + j) : 1.0f, sbp);
+                                (int32_t)vals[first + j] >> SHIFT, scale_a ? ld_behind_wait(scale_a + q_first + j) : 1.0f, sbp);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)

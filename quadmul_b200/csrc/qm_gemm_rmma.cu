@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t word(const uint4 &v, int s) { return s == 0 
 // through the reduction.
 template <int WARPS, int RG, int MS, int MODE, bool TOK8>
 __global__ void __launch_bounds__(WARPS * 32, (WARPS == 16 ? 1 : 2))
-gemm_rmma_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, int32_t *__restrict__ C, int64_t ldc, int m, int n, int k,
-                 uint16_t *__restrict__ out_bf16, const float *__restrict__ scale_a, const float *__restrict__ scale_b)
+gemm_rmma_kernel(const uint8_t *A, const uint8_t *B, int32_t *C, int64_t ldc, int m, int n, int k,
+                 uint16_t *out_bf16, const float *scale_a, const float *scale_b)
 {
     using Cfg = RmmaCfg<WARPS, RG, MS>;
     constexpr int kWarps = Cfg::kWarps, kThreads = Cfg::kThreads, kRowGroups = Cfg::kRowGroups, kRowsPerCta = Cfg::kRowsPerCta,
@@ -144,7 +144,7 @@ gemm_rmma_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, i
         for (int i = threadIdx.x; i < 16 * tiles * chunks; i += kThreads) {
             const int r = i / chunks, c = i - r * chunks;
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < m) v = __ldg(reinterpret_cast<const uint4 *>(A + (int64_t)r * row_bytes) + c);
+            if (r < m) v = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(A + (int64_t)r * row_bytes) + c);
             a_pk[r * pk_stride + c] = v;
         }
         __syncthreads();
@@ -157,7 +157,7 @@ gemm_rmma_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, i
 #pragma unroll
             for (int u = 0; u < kMaxSteps; ++u)
 #pragma unroll
-                for (int rg = 0; rg < kRowGroups; ++rg) w[u][rg] = __ldcs(src + 32 * (u * kRowGroups + rg));
+                for (int rg = 0; rg < kRowGroups; ++rg) w[u][rg] = ptx::ldcs_behind_wait(src + 32 * (u * kRowGroups + rg));
         } else if constexpr (WIDE) {
 #pragma unroll
             for (int rg = 0; rg < kRowGroups; ++rg) {
@@ -176,10 +176,10 @@ gemm_rmma_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, i
                 for (int rg = 0; rg < kRowGroups; ++rg) {
                     const int row = rb * kRowsPerCta + rg * 8 + g;
                     if constexpr (FULL) {
-                        w[u][rg] = __ldcs(reinterpret_cast<const uint4 *>(B + (int64_t)row * row_bytes) + c);
+                        w[u][rg] = ptx::ldcs_behind_wait(reinterpret_cast<const uint4 *>(B + (int64_t)row * row_bytes) + c);
                     } else {
                         w[u][rg] = make_uint4(0, 0, 0, 0);
-                        if (t < steps && c < chunks && row < n) w[u][rg] = __ldcs(reinterpret_cast<const uint4 *>(B + (int64_t)row * row_bytes) + c);
+                        if (t < steps && c < chunks && row < n) w[u][rg] = ptx::ldcs_behind_wait(reinterpret_cast<const uint4 *>(B + (int64_t)row * row_bytes) + c);
                     }
                 }
             }
@@ -268,7 +268,7 @@ gemm_rmma_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, i
         if (mine && token < m && p < n) {
             if (out_bf16)
                 out_bf16[(int64_t)token * ldc + p] =
-                    (uint16_t)dequant_bf16_bits(sum, scale_a ? __ldg(scale_a + token) : 1.0f, scale_b ? __ldg(scale_b + p) : 1.0f);
+                    (uint16_t)dequant_bf16_bits(sum, scale_a ? ptx::ld_behind_wait(scale_a + token) : 1.0f, scale_b ? ptx::ld_behind_wait(scale_b + p) : 1.0f);
             else
                 C[(int64_t)token * ldc + p] = sum;
         }

@@ -129,8 +129,8 @@ template <int H, bool MC, bool DQ>
 __global__ void __launch_bounds__(kNumThreads, 1)
 gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB,
                 const __grid_constant__ CUtensorMap tmapC, int use_tma_store, int32_t *__restrict__ C, int64_t ldc, int M,
-                int N, int K, int *status, int split_k, int tail_tiles, int tail_split, const float *__restrict__ scale_a,
-                const float *__restrict__ scale_b)
+                int N, int K, int *status, int split_k, int tail_tiles, int tail_split, const float *scale_a,
+                const float *scale_b)
 {
     using Cfg = Tc2Cfg<H>;
     constexpr int S = Cfg::S, SP = Cfg::SP;
@@ -327,12 +327,12 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
             if constexpr (DQ) {
                 // this lane's row scale and, spread over the lanes, the scales of the warp's 128 columns
                 const int row = row0 + lane;
-                const float sa = (scale_a && row < M) ? __ldg(scale_a + row) : 1.0f;
+                const float sa = (scale_a && row < M) ? ld_behind_wait(scale_a + row) : 1.0f;
                 float sb[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int col = q0 + 32 * i + lane;
-                    sb[i] = (scale_b && col < N) ? __ldg(scale_b + col) : 1.0f;
+                    sb[i] = (scale_b && col < N) ? ld_behind_wait(scale_b + col) : 1.0f;
                 }
                 tmem_ld_x32(taddr, va);
                 tmem_ld_x32(taddr + 32, vb);

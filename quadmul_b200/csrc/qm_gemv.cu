@@ -35,8 +35,8 @@ constexpr int kWarps = kThreads / 32;
 // when the stream is long: 4 x 28672 x 8192 35 against 43 us); the launcher picks by n.
 template <int MR, int RU>
 __global__ void __launch_bounds__(kThreads)
-gemv_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, int32_t *__restrict__ C, int64_t ldc, int m, int n, int k,
-            uint16_t *__restrict__ out_bf16, const float *__restrict__ scale_a, const float *__restrict__ scale_b)
+gemv_kernel(const uint8_t *A, const uint8_t *B, int32_t *C, int64_t ldc, int m, int n, int k,
+            uint16_t *out_bf16, const float *scale_a, const float *scale_b)
 {
     extern __shared__ uint4 a_cv[];  // [MR][chunks][2]: even elements x 16, odd elements x 16 of each 16-byte chunk of A
     ptx::grid_launch_dependents();
@@ -68,7 +68,7 @@ gemv_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, int32_
     for (int i = threadIdx.x; i < MR * chunks; i += kThreads) {
         const int r = i / chunks, c = i - r * chunks;
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (r < m) w = __ldg(reinterpret_cast<const uint4 *>(A + r * row_bytes) + c);
+        if (r < m) w = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(A + r * row_bytes) + c);
         uint4 lo, hi;
         tc::split_s4x32(w, lo, hi);
         a_cv[2 * i] = lo;
@@ -112,7 +112,7 @@ gemv_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, int32_
         for (int c = lane; c < chunks; c += 32) {
             uint4 w[kRowsPerStep];
 #pragma unroll
-            for (int u = 0; u < kRowsPerStep; ++u) w[u] = __ldcs(brow[u] + c);
+            for (int u = 0; u < kRowsPerStep; ++u) w[u] = ptx::ldcs_behind_wait(brow[u] + c);
             accumulate(c, w);
         }
 #pragma unroll
@@ -138,7 +138,7 @@ gemv_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ B, int32_
                 s >>= 8;
                 if (out_bf16)
                     out_bf16[(int64_t)r * ldc + p] =
-                        (uint16_t)dequant_bf16_bits(s, scale_a ? __ldg(scale_a + r) : 1.0f, scale_b ? __ldg(scale_b + p) : 1.0f);
+                        (uint16_t)dequant_bf16_bits(s, scale_a ? ptx::ld_behind_wait(scale_a + r) : 1.0f, scale_b ? ptx::ld_behind_wait(scale_b + p) : 1.0f);
                 else
                     C[(int64_t)r * ldc + p] = s;
             }

@@ -344,6 +344,49 @@ __device__ __forceinline__ void grid_dependency_wait()
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Loads for kernels that may begin while the kernel before still runs.  A read-only load (__ldg, or one through const __restrict__)
+// promises that nothing writes the memory as long as the kernel lives, and may be moved in front of the wait; so may the
+// intrinsics with a cache hint.  These are ordinary loads that stay behind it: volatile statements keep their order.
+__device__ __forceinline__ uint4 ld_behind_wait(const uint4 *p)
+{
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ld_behind_wait(const uint2 *p)
+{
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_behind_wait(const uint32_t *p)
+{
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ unsigned short ld_behind_wait(const unsigned short *p)
+{
+    unsigned short v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_behind_wait(const uint8_t *p)
+{
+    uint32_t v;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int ld_behind_wait(const int *p) { return (int)ld_behind_wait(reinterpret_cast<const uint32_t *>(p)); }
+__device__ __forceinline__ float ld_behind_wait(const float *p) { return __uint_as_float(ld_behind_wait(reinterpret_cast<const uint32_t *>(p))); }
+// the same for what is read once (evicted first)
+__device__ __forceinline__ uint4 ldcs_behind_wait(const uint4 *p)
+{
+    uint4 v;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ uint32_t cluster_ctarank()
 {
     uint32_t r;

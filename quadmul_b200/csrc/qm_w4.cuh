@@ -6,6 +6,7 @@
 #include <cstdlib>
 
 #include "qm_internal.h"
+#include "qm_ptx.cuh"
 
 namespace qm {
 namespace w4 {
@@ -13,6 +14,14 @@ namespace w4 {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// *p as fp32, by a load that stays behind the wait for the kernel before
+__device__ __forceinline__ float load_float(const float *p) { return ptx::ld_behind_wait(p); }
+__device__ __forceinline__ float load_float(const __half *p) { return __half2float(__ushort_as_half(ptx::ld_behind_wait(reinterpret_cast<const unsigned short *>(p)))); }
+__device__ __forceinline__ float load_float(const __nv_bfloat16 *p)
+{
+    return __uint_as_float((uint32_t)ptx::ld_behind_wait(reinterpret_cast<const unsigned short *>(p)) << 16);
+}
 
 template <typename T>
 __device__ __forceinline__ T from_float(float v);  // one rounding, to nearest even
@@ -51,7 +60,8 @@ int with_same_or_float(int other, F f)
 }
 
 // Launch that may begin while the previous kernel of the stream still runs: the kernel waits (griddepcontrol.wait) before it
-// touches global memory.  QM_NO_PDL=1 turns that off.
+// touches global memory, reads it with loads that stay behind the wait (ptx::ld_behind_wait), and lets its own successor begin
+// only then, so that no kernel is resident while the last but one before it still runs.  QM_NO_PDL=1 turns that off.
 template <typename... P, typename... A>
 int launch_chained(const char *what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t stream, A... args)
 {
@@ -102,12 +112,12 @@ __device__ __forceinline__ bool elect_one()
 // The experts' segments, from offsets that may be anything: seg[e] (e = 0 .. experts) is the running maximum of the offsets
 // clamped to [0, rows], so expert e has the rows [seg[e], seg[e + 1]); tiles[e] is how many tiles of `tile` rows the experts
 // below e have.  Run by one warp; seg and tiles are shared memory, to be read after a barrier.
-__device__ __forceinline__ void scan_segments(const int *__restrict__ offsets, int experts, int rows, int tile, int *seg, int *tiles, int lane)
+__device__ __forceinline__ void scan_segments(const int *offsets, int experts, int rows, int tile, int *seg, int *tiles, int lane)
 {
     int top = 0, sum = 0;  // running maximum and sum of what came before
     for (int base = 0; base <= experts; base += 32) {
         const int e = base + lane;
-        int v = e <= experts ? max(0, min(__ldg(offsets + e), rows)) : 0;
+        int v = e <= experts ? max(0, min(ptx::ld_behind_wait(offsets + e), rows)) : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(0xFFFFFFFFu, v, d);

@@ -16,11 +16,11 @@ constexpr int kThreads = 256;
 // rows x row_bytes from `src` (pitch src_pitch, any alignment) to rows of dst_pitch bytes (a multiple of 16) on 16-byte boundaries;
 // zeros behind row_bytes.  A thread makes 16 bytes out of aligned words, shifted into place; where a word of the shift would lie
 // outside the matrix (its first and last bytes) it takes single bytes.
-__global__ void __launch_bounds__(kThreads) w4_pad_kernel(const uint8_t *__restrict__ src, int64_t src_pitch, int64_t row_bytes, uint8_t *__restrict__ dst,
+__global__ void __launch_bounds__(kThreads) w4_pad_kernel(const uint8_t *src, int64_t src_pitch, int64_t row_bytes, uint8_t *dst,
                                                           int dst_pitch, int64_t rows)
 {
-    ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int pieces = dst_pitch / 16;
     const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = begin + (rows - 1) * src_pitch + row_bytes;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * kThreads) {
@@ -32,30 +32,30 @@ __global__ void __launch_bounds__(kThreads) w4_pad_kernel(const uint8_t *__restr
         if (here == 16 && words >= begin && words + 20 <= end) {
             uint32_t w[5];
 #pragma unroll
-            for (int j = 0; j < 5; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t *>(words) + j);
+            for (int j = 0; j < 5; ++j) w[j] = ptx::ld_behind_wait(reinterpret_cast<const uint32_t *>(words) + j);
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], 8 * (int)(from & 3));
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                if (j < here) o[j >> 2] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t *>(from) + j) << (8 * (j & 3));
+                if (j < here) o[j >> 2] |= ptx::ld_behind_wait(reinterpret_cast<const uint8_t *>(from) + j) << (8 * (j & 3));
         }
         *reinterpret_cast<uint4 *>(dst + row * dst_pitch + at) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
 // zeros in the rows of out that some expert has (all rows without offsets): a block per row
-__global__ void __launch_bounds__(kThreads) w4_zero_kernel(unsigned short *__restrict__ out, int64_t ldo, const int *__restrict__ offsets, int experts, int rows,
+__global__ void __launch_bounds__(kThreads) w4_zero_kernel(unsigned short *out, int64_t ldo, const int *offsets, int experts, int rows,
                                                            int n)
 {
-    ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     if (offsets) {
         // the experts' segments cover what lies between the first offset and the largest, both clamped
         const int row = (int)blockIdx.x;
         bool before = false, behind = false;
         for (int e = threadIdx.x; e <= experts; e += kThreads) {
-            const int o = max(0, min(__ldg(offsets + e), rows));
+            const int o = max(0, min(ptx::ld_behind_wait(offsets + e), rows));
             before |= e == 0 && row < o;
             behind |= row < o;
         }

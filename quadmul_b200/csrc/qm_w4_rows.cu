@@ -128,11 +128,11 @@ __device__ __noinline__ float plain_output(const T *x, const uint8_t *b, const S
     for (int g0 = 0, g = 0; g0 < k; g0 += group, ++g) {
         float part = 0.0f;
         for (int i = g0; i < min(k, g0 + group); i += 2) {
-            const int byte = (int8_t)b[i >> 1];
-            part = fmaf(to_float(x[i]), (float)((int)((uint32_t)byte << 28) >> 28), part);
-            part = fmaf(to_float(x[i + 1]), (float)(byte >> 4), part);
+            const int byte = (int8_t)ptx::ld_behind_wait(b + (i >> 1));
+            part = fmaf(load_float(x + i), (float)((int)((uint32_t)byte << 28) >> 28), part);
+            part = fmaf(load_float(x + i + 1), (float)(byte >> 4), part);
         }
-        sum = fmaf(to_float(s[g]), part, sum);
+        sum = fmaf(load_float(s + g), part, sum);
     }
     return sum;
 }
@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
     constexpr int kColumns = 8;
     constexpr int kPlace = 2 * TT * 32;            // 16-byte pieces of X per step
     extern __shared__ uint4 smem_u4[];
-    const T *__restrict__ X = static_cast<const T *>(p.X);
-    const S *__restrict__ scales = static_cast<const S *>(p.scales);
+    const T *X = static_cast<const T *>(p.X);
+    const S *scales = static_cast<const S *>(p.scales);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int groups_of_rows = kWarps / p.warps_k;
     const int wk = warp % p.warps_k, wr = warp / p.warps_k;
@@ -167,7 +167,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
     unsigned *odd_rows = reinterpret_cast<unsigned *>(red + 2 * kRedFloats);  // [pair's parity][kWarps]
     int *seg = reinterpret_cast<int *>(odd_rows + 2 * kWarps), *tiles = seg + p.experts + 1;
 
-    ptx::grid_launch_dependents();
     // CTA c takes the units from first_unit(c) up to first_unit(c + 1); the host has seen to it that their number fits an int
     auto first_unit = [&](int units, unsigned c) {
         const unsigned each = (unsigned)units / gridDim.x, more = (unsigned)units % gridDim.x;
@@ -180,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
         if (row < p.n) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.B + (int64_t)row * row_bytes), "r"(row_bytes) : "memory");
     }
     ptx::grid_dependency_wait();  // nothing above read or wrote global memory
+    ptx::grid_launch_dependents();
 
     int pairs = row_tiles;  // (expert, tile of rows)
     if (p.offsets) {
@@ -228,22 +228,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
         const int t = wk + lw.step * p.warps_k;
         const uint8_t *src = lb + (4 * t + q < chunks ? t * 64 + q * 16 : 0);  // beyond K the codes meet zeros
 #pragma unroll
-        for (int r = 0; r < kRG; ++r) b.w[r] = __ldcs(reinterpret_cast<const uint4 *>(src + lrow[r]));
+        for (int r = 0; r < kRG; ++r) b.w[r] = ptx::ldcs_behind_wait(reinterpret_cast<const uint4 *>(src + lrow[r]));
         using Raw = RawScales<S, GPS>;
         const int first = GPS > 1 ? t * GPS : (t * kStep) >> p.group_shift;
         if (t >= steps) {
 #pragma unroll
             for (int j = 0; j < Raw::kWords; ++j) b.s.w[j] = 0;
         } else if constexpr (GPS == 1) {
-            if constexpr (sizeof(S) == 4) b.s.w[0] = __float_as_uint(to_float(__ldg(sp + first)));
-            else b.s.w[0] = __ldg(reinterpret_cast<const unsigned short *>(sp + first));
+            if constexpr (sizeof(S) == 4) b.s.w[0] = __float_as_uint(load_float(sp + first));
+            else b.s.w[0] = ptx::ld_behind_wait(reinterpret_cast<const unsigned short *>(sp + first));
         } else if (p.vec_scales) {
-            if constexpr (Raw::kWords == 1) b.s.w[0] = __ldg(reinterpret_cast<const uint32_t *>(sp + first));
+            if constexpr (Raw::kWords == 1) b.s.w[0] = ptx::ld_behind_wait(reinterpret_cast<const uint32_t *>(sp + first));
             else if constexpr (Raw::kWords == 2) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(sp + first));
+                const uint2 v = ptx::ld_behind_wait(reinterpret_cast<const uint2 *>(sp + first));
                 b.s.w[0] = v.x, b.s.w[1] = v.y;
             } else {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(sp + first));
+                const uint4 v = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(sp + first));
                 b.s.w[0] = v.x, b.s.w[1] = v.y, b.s.w[2] = v.z, b.s.w[3] = v.w;
             }
         } else {
@@ -252,8 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
 #pragma unroll
             for (int j = 0; j < GPS; ++j) {
                 if (first + j >= p.groups) continue;
-                if constexpr (sizeof(S) == 4) b.s.w[j] = __float_as_uint(to_float(__ldg(sp + first + j)));
-                else b.s.w[j >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(sp + first + j)) << (16 * (j & 1));
+                if constexpr (sizeof(S) == 4) b.s.w[j] = __float_as_uint(load_float(sp + first + j));
+                else b.s.w[j >> 1] |= (uint32_t)ptx::ld_behind_wait(reinterpret_cast<const unsigned short *>(sp + first + j)) << (16 * (j & 1));
             }
         }
         advance(lw);
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
             for (int r = 0; r < kTile / 2; ++r) {
                 ahead[r] = make_uint4(0, 0, 0, 0);
                 if (i < mine && 2 * r + side < tokens && at < p.k)
-                    ahead[r] = __ldg(reinterpret_cast<const uint4 *>(X + (int64_t)(first_row + 2 * r + side) * p.ldx + at));
+                    ahead[r] = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(X + (int64_t)(first_row + 2 * r + side) * p.ldx + at));
             }
         };
         fetch(wr);

@@ -149,7 +149,7 @@ __device__ __forceinline__ uint32_t cluster_nctarank()
 // The power of two below a row's largest scale (1 for a row of zeros or with a scale that is not finite); bf16 has fp32's range
 // and needs none.
 template <typename T, typename S>
-__device__ __forceinline__ float row_unit(const S *__restrict__ s, int groups)
+__device__ __forceinline__ float row_unit(const S *s, int groups)
 {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         return 1.0f;
@@ -164,7 +164,7 @@ __device__ __forceinline__ float row_unit(const S *__restrict__ s, int groups)
             for (int j = 0; j <= last; j += kAhead) {
                 uint4 u[kAhead];
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) u[i] = __ldg(v + min(j + i, last));
+                for (int i = 0; i < kAhead; ++i) u[i] = ld_behind_wait(v + min(j + i, last));
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
                     const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
@@ -182,7 +182,7 @@ __device__ __forceinline__ float row_unit(const S *__restrict__ s, int groups)
             for (int j = 0; j < groups; j += 4 * kAhead) {
                 uint32_t u[4 * kAhead];
 #pragma unroll
-                for (int i = 0; i < 4 * kAhead; ++i) u[i] = __ldg(v + min(j + i, groups - 1));
+                for (int i = 0; i < 4 * kAhead; ++i) u[i] = ld_behind_wait(v + min(j + i, groups - 1));
 #pragma unroll
                 for (int i = 0; i < 4 * kAhead; ++i) most = max(most, u[i] & (sizeof(S) == 4 ? 0x7FFFFFFFu : 0x7FFFu));
             }
@@ -221,7 +221,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
     float *unit_of_row = reinterpret_cast<float *>(generic0 + 8 * kNumBarriers + 16);
     int *seg = reinterpret_cast<int *>(unit_of_row + kRowsB), *tiles = seg + p.experts + 1;
 
-    grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();                  // half of the pair, or part of K
     const int parts = G == 1 ? (int)cluster_nctarank() : 1;   // parts of K
@@ -250,6 +249,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
     if (p.offsets && warp == 3) scan_segments(p.offsets, p.experts, p.rows, p.tile, seg, tiles, lane);
     tc_fence_before_sync();
     __syncthreads();
+    grid_launch_dependents();  // (the TMEM is taken by now: a successor that wants some waits for this kernel, not the other way round)
     if (G == 2) {  // the pair's barriers are there (in the SPLIT form a CTA keeps to itself until the parts are added up)
         cluster_arrive();
         cluster_wait();
@@ -406,7 +406,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
         const int set = (warp - kConvWarp) >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;              // row of this CTA's part of B = TMEM lane
         const uint32_t swz = (uint32_t)((r >> 1) & 3);  // 64-byte TMA swizzle: chunk ^= (row / 2) % 4
-        const S *__restrict__ scales = static_cast<const S *>(p.scales);
+        const S *scales = static_cast<const S *>(p.scales);
         uint32_t it = 0;
         bool ok = true;
         for (int t = cluster; t < num_items && ok; t += clusters) {
@@ -420,24 +420,24 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
             auto load_scales = [&](int kb, float(&v)[4]) {
                 const int first = (kb * kStageK) >> p.group_shift;
                 if (p.group_shift >= 7) {
-                    v[0] = v[1] = v[2] = v[3] = to_float(sp[first]);
+                    v[0] = v[1] = v[2] = v[3] = load_float(sp + first);
                 } else if (p.vec_scales) {
                     if (p.group_shift == 6) {
                         const S *a = sp + first;
                         if constexpr (sizeof(S) == 4) {
-                            const float2 u = __ldg(reinterpret_cast<const float2 *>(a));
-                            v[0] = v[1] = u.x, v[2] = v[3] = u.y;
+                            const uint2 u = ld_behind_wait(reinterpret_cast<const uint2 *>(a));
+                            v[0] = v[1] = __uint_as_float(u.x), v[2] = v[3] = __uint_as_float(u.y);
                         } else {
-                            const float2 u = unpack2(__ldg(reinterpret_cast<const uint32_t *>(a)), Tag<T>());
+                            const float2 u = unpack2(ld_behind_wait(reinterpret_cast<const uint32_t *>(a)), Tag<T>());
                             v[0] = v[1] = u.x, v[2] = v[3] = u.y;
                         }
                     } else {
                         const S *a = sp + first;
                         if constexpr (sizeof(S) == 4) {
-                            const float4 u = __ldg(reinterpret_cast<const float4 *>(a));
-                            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+                            const uint4 u = ld_behind_wait(reinterpret_cast<const uint4 *>(a));
+                            v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
                         } else {
-                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(a));
+                            const uint2 u = ld_behind_wait(reinterpret_cast<const uint2 *>(a));
                             const float2 lo = unpack2(u.x, Tag<T>()), hi = unpack2(u.y, Tag<T>());
                             v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
                         }
@@ -446,7 +446,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int g = (kb * kStageK + 32 * j) >> p.group_shift;
-                        v[j] = g < p.groups ? to_float(sp[g]) : 0.0f;
+                        v[j] = g < p.groups ? load_float(sp + g) : 0.0f;
                     }
                 }
             };
@@ -521,8 +521,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
         // ------------------------------ epilogue ------------------------------
         const int quarter = warp & 3, half = (warp - kEpiWarp) >> 2;
         const int r = quarter * 32 + lane;
-        const S *__restrict__ scales = static_cast<const S *>(p.scales);
-        T *__restrict__ out = static_cast<T *>(p.out);
+        const S *scales = static_cast<const S *>(p.scales);
+        T *out = static_cast<T *>(p.out);
         uint32_t lt = 0;
         for (int t = cluster; t < num_items; t += clusters, ++lt) {
             const Item m = item(t);
@@ -607,7 +607,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ 
             if (cluster < num_items) {
                 // this CTA finishes every parts-th row of the tile; a thread two neighbouring columns of a row at a time
                 const Item m = item(cluster);
-                T *__restrict__ out = static_cast<T *>(p.out);
+                T *out = static_cast<T *>(p.out);
                 const int todo = (m.count - rank + parts - 1) / parts;
                 for (int i = threadIdx.x; i < todo * (kRowsB / 2); i += kNumThreads) {
                     const int row = rank + (i / (kRowsB / 2)) * parts, pos = (i % (kRowsB / 2)) * 2, col = m.col + pos;
