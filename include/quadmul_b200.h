@@ -281,8 +281,13 @@ typedef enum qm_type {
 /*
  * X (m x k, row pitch ldx elements) times the transpose of B into out (m x n, row pitch ldo elements); X and out are both
  * QM_TYPE_F16 or both QM_TYPE_BF16 (`type`), the scales have that type or QM_TYPE_F32, group is 32, 64, 128 or 256, k is even.
- * Sums are fp32 and are rounded to `type` once; with many rows a weight scale * q is rounded to `type` before it is multiplied
- * (fp16: relative to the largest scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).  A scale
+ * Sums are fp32 and are rounded to `type` once.  Beside that an element or a weight is rounded, by the number of rows:
+ *   up to 8 rows (on average per expert), where they fit the kernel for few rows: X is read to 22 bits below the largest of its (at
+ *   most 128) neighbours under one scale; a row in which more than a quarter of the elements of such a stretch would lose digits is
+ *   summed in fp32 as it is.
+ *   otherwise: a weight scale * q is rounded to `type` before it is multiplied, by at most half a step (fp16: relative to the largest
+ *   scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).
+ * So the last place of a row's result can depend on how many rows the call has.  A scale
  * that is not finite makes its column not finite; QM_TYPE_BF16 counts scales from 2^126 on among them.  out is fully overwritten;
  * k == 0 zeroes it, k is at most 2^30 - 32.  n * experts is below 2^31 - 512.  out shares no element with the inputs, here and below.
  *   k % 32 == 0, ldx % 8 == 0 and 16-byte-aligned X and B need no workspace.  Otherwise X and B are copied into one (device

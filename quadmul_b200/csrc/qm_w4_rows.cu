@@ -10,7 +10,11 @@
 //   are exact in int32 (mma.sync.m16n8k32), and scale * (d1 . q, d2 . q, d3 . q) is added in fp32, one rounding per stretch, as
 //   an fp32 sum of products would have one per product.  The only loss is that of elements below 2^-13 of their stretch's largest
 //   (bf16; 2^-10 for fp16): their last bits are rounded at 2^-22 of it, four times fp32's own last place.
-//   A row with an infinity or a NaN cannot be written so; its outputs are computed again, element by element.
+//   That is nothing beside the other elements' products, but a weight of zero can take the largest one out of a sum.  So where more
+//   than a quarter of a stretch's elements lose digits (an element hundreds, fp16, or thousands of times its neighbours), or one is an
+//   infinity or a NaN, the row's outputs are computed from their definition instead, element by element: 1 x 4096 x 4096 14 us,
+//   8 x 4096 x 4096 58 us with all rows so.  Finding out costs a vote per 256 elements of X, and a count (8 x 4096 x 4096 8.2 -> 10.2
+//   us) only where eight neighbours have nothing above 2^-8 of their stretch's largest.
 //
 //  * A CTA (16 warps) takes blocks of 32 rows of B per warp group; WK of its warps split K between them in steps of 128 elements.
 //    Lane (g, q) = (lane / 4, lane % 4) loads 16 bytes, 32 codes, of row g of each 8-row group straight into registers; kDepth steps
@@ -120,21 +124,88 @@ __device__ __forceinline__ bool barrier_or(int id, int threads, bool any)
     return r != 0;
 }
 
-// One output from its definition, in the order of K.
+// Element j of eight 16-bit floats
+template <typename T>
+__device__ __forceinline__ float element(const uint4 &v, int j)
+{
+    const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)((j & 1) ? w >> 16 : w)));
+    else return __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
+}
+
+// The eight codes of a word as fp32: nibble n is (n ^ 8) - 8, and n ^ 8 in the last bits of 2^23 reads as 2^23 + (n ^ 8).
+__device__ __forceinline__ float code_as_float(uint32_t w, int j) { return __fadd_rn(__uint_as_float(and_xor(w >> (4 * j), 0xFu, 0x4B000008u)), -8388616.0f); }
+
+// A thread's share of one output from its definition: pieces `part`, `part` + `parts`, ... of 32 elements of K (X and B are such that these
+// are aligned, and no group ends inside one).  It takes few registers: what the caller has on the way stays in its own.
 template <typename T, typename S>
-__device__ __noinline__ float plain_output(const T *x, const uint8_t *b, const S *s, int k, int group)
+__device__ __noinline__ float plain_part(const T *x, const uint8_t *b, const S *s, int k, int group_shift, int part, int parts)
 {
     float sum = 0.0f;
-    for (int g0 = 0, g = 0; g0 < k; g0 += group, ++g) {
-        float part = 0.0f;
-        for (int i = g0; i < min(k, g0 + group); i += 2) {
-            const int byte = (int8_t)ptx::ld_behind_wait(b + (i >> 1));
-            part = fmaf(load_float(x + i), (float)((int)((uint32_t)byte << 28) >> 28), part);
-            part = fmaf(load_float(x + i + 1), (float)(byte >> 4), part);
+    for (int i = part * 32; i < k; i += parts * 32) {
+        uint4 w = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(b + i / 2));
+        const float scale = load_float(s + (i >> group_shift));
+        float even = 0.0f, odd = 0.0f;
+#pragma unroll 1
+        for (int o = 0; o < 4; ++o) {
+            const uint4 e = ptx::ld_behind_wait(reinterpret_cast<const uint4 *>(x + i) + o);
+            const uint32_t codes = w.x;
+            w.x = w.y, w.y = w.z, w.z = w.w;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                even = fmaf(element<T>(e, j), code_as_float(codes, j), even);
+                odd = fmaf(element<T>(e, j + 1), code_as_float(codes, j + 1), odd);
+            }
         }
-        sum = fmaf(load_float(s + g), part, sum);
+        sum = fmaf(scale, even + odd, sum);
     }
     return sum;
+}
+
+// The largest magnitudes of the even and the odd ones of eight elements, as the bits of T: these order like numbers.
+__device__ __forceinline__ uint32_t magnitudes(const uint4 &v)
+{
+    return __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+}
+
+// How a stretch is scaled, from the bits of its largest magnitude.
+struct Stretch {
+    uint32_t e, ec;  // biased exponent: the largest is below 2^(e - 126); as it is used (below 2^-101 the bits run out early)
+    __device__ __forceinline__ float up() const { return __uint_as_float((274u - ec) << 23); }  // 2^21 over the power of two above the largest
+    __device__ __forceinline__ float down() const { return __uint_as_float((ec - 20u) << 23); }  // one over that
+};
+template <typename T>
+__device__ __forceinline__ Stretch stretch_of(uint32_t m)
+{
+    float top;
+    if constexpr (std::is_same<T, __half>::value) top = __half2float(__ushort_as_half((unsigned short)m));
+    else top = __uint_as_float(m << 16);
+    Stretch s;
+    s.e = __float_as_uint(top) >> 23;
+    s.ec = min(max(s.e, 25u), 254u);
+    return s;
+}
+
+// Whether the stretch that LANES neighbouring lanes have eight elements of each cannot be written as bytes: one is not finite, or more
+// than a quarter of those that are not zero lose digits.  The whole warp.  These are counted only where some lane of it has nothing
+// above 2^-8 of its stretch's largest (m; `here` is the lane's own).
+template <typename T, int LANES>
+__device__ __forceinline__ bool loses_digits(const uint4 &v, uint32_t here, uint32_t m, const Stretch &s)
+{
+    constexpr uint32_t kOctaves = std::is_same<T, __half>::value ? 8u << 10 : 8u << 7;  // in the exponent: a factor of 2^8
+    bool bad = s.e == 255u;
+    if (__any_sync(0xFFFFFFFFu, here != 0u && (here + kOctaves < m || s.e < 25u))) {
+        int count = 0;  // elements that are not zero, and in the upper half those that lose digits
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = element<T>(v, j);
+            count += (x != 0.0f ? 1 : 0) + (__fmul_rn(rintf(x * s.up()), s.down()) != x ? 1 << 16 : 0);
+        }
+#pragma unroll
+        for (int d = 1; d < LANES; d <<= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, d);
+        bad |= 4 * (count >> 16) > (count & 0xFFFF);
+    }
+    return bad;
 }
 
 // GPS = groups per step of 128 elements (4, 2 or 1 for groups of 32, 64, and 128 or more).
@@ -159,8 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
     const int mine = max(1, (steps - wk + p.warps_k - 1) / p.warps_k);
     const int places = max(steps, p.warps_k);
 
-    // X [place][pair of sets][instruction][lane] 16 bytes, X's units [place][group][column], partial tiles, rows of X that are not
-    // finite, segments
+    // X [place][pair of sets][instruction][lane] 16 bytes, X's units [place][group][column], partial tiles, rows of X that
+    // bytes do not hold, segments
     uint4 *xs = smem_u4;
     float *unit = reinterpret_cast<float *>(smem_u4 + (size_t)places * kPlace);
     float *red = unit + (size_t)places * GPS * kColumns;
@@ -262,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) load(buf[d]);
 
-    unsigned bad_rows = 0;  // rows of X with an element that is not finite, as far as this warp has seen
+    unsigned bad_rows = 0;  // rows of X that bytes do not hold, as far as this warp has seen
     bool staged_bad = false, cpair_seen = false;
     int parity = 0, pair_parity = 0, first_row = 0, tokens = 0, cpair = -1;
     float acc[kTiles][4];
@@ -296,26 +367,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
             for (int r = 0; r < kTile / 2; ++r) {
                 const int row = 2 * r + side;
                 if (2 * r >= tokens) continue;  // (columns without a row hold anything: nobody reads their sums)
-                uint32_t m = __vmaxu2(__vmaxu2(v[r].x & 0x7FFF7FFFu, v[r].y & 0x7FFF7FFFu), __vmaxu2(v[r].z & 0x7FFF7FFFu, v[r].w & 0x7FFF7FFFu));
+                uint32_t m = magnitudes(v[r]);
+                const uint32_t here = max(m & 0xFFFFu, m >> 16);
 #pragma unroll
                 for (int d = 1; d < 16 / GPS; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
                 m = max(m & 0xFFFFu, m >> 16);
-                float top;
-                if constexpr (std::is_same<T, __half>::value) top = __half2float(__ushort_as_half((unsigned short)m));
-                else top = __uint_as_float(m << 16);
-                const uint32_t e = __float_as_uint(top) >> 23;  // biased exponent: top < 2^(e - 126)
-                if (e == 255u) bad |= 1u << row;
-                const uint32_t ec = min(max(e, 25u), 254u);      // (below 2^-101 the bits run out early)
-                const float up = __uint_as_float((274u - ec) << 23);  // 2^21 over the power of two above top
+                const Stretch st = stretch_of<T>(m);
+                if (loses_digits<T, 16 / GPS>(v[r], here, m, st)) bad |= 1u << row;
                 uint32_t z[8];
-                const uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float x;
-                    if constexpr (std::is_same<T, __half>::value) x = __half2float(__ushort_as_half((unsigned short)((j & 1) ? w[j >> 1] >> 16 : w[j >> 1])));
-                    else x = __uint_as_float((j & 1) ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
                     // 1.5 x 2^23 rounds to a whole number; 128 more in the two low digits makes their bytes unsigned
-                    z[j] = __float_as_uint(fmaf(x, up, 12582912.0f + 32896.0f));
+                    z[j] = __float_as_uint(fmaf(element<T>(v[r], j), st.up(), 12582912.0f + 32896.0f));
                 }
                 // even elements 0, 2, 4, 6 and odd elements 1, 3, 5, 7: their bytes 0 (d3 + 128), 1 (d2 + 128) and 2 (d1 + 64)
                 uint32_t d[3][2];
@@ -327,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
                     const uint32_t c = __byte_perm(__byte_perm(z[o], z[2 + o], 0x0062), __byte_perm(z[4 + o], z[6 + o], 0x0062), 0x5410);
                     d[0][o] = ((c | 0x80808080u) - 0x40404040u) ^ 0x80808080u;
                 }
-                const float f = __uint_as_float((ec - 24u) << 23);  // one over up, and over the codes' factor of 16
+                const float f = __uint_as_float((st.ec - 24u) << 23);  // one over up, and over the codes' factor of 16
                 const bool lead = (word & (16 / GPS - 1)) == 0;
                 const int j = GPS == 1 ? 0 : GPS == 2 ? word >> 3 : word >> 2;
                 uint2 *dst = reinterpret_cast<uint2 *>(xs + t * kPlace + (s >> 1) * TT * 32) + (s & 1);
@@ -438,21 +501,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
             for (int w = 0; w < 8; ++w)
                 if (w < p.warps_k) sum += src[w * kTiles * 128];
             if (!WIDE && b == 3) sum = 0.0f;
+            const int col = cw.block * block_rows + wr * kRows + r;
+            if (any_bad && o < todo && col < p.n) {
+                unsigned bad = 0;
+                for (int w = 0; w < kWarps; ++w) bad |= odd_rows[pair_parity * kWarps + w];
+                if (bad >> tok & 1) {  // the threads that share the output share K instead
+                    const int64_t brow = (int64_t)cw.expert * p.n + col;
+                    sum = plain_part(X + (int64_t)(first_row + tok) * p.ldx, p.B + brow * (p.k / 2), scales + brow * p.groups, p.k, p.group_shift,
+                                     o & ((1 << share_bits) - 1), 1 << share_bits);
+                }
+            }
             if constexpr (!WIDE) {
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
             }
             if (p.warps_k == 16) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, WIDE ? 1 : 4);
-            const int col = cw.block * block_rows + wr * kRows + r;
             if (o >= todo || (o & ((1 << share_bits) - 1)) != 0 || col >= p.n) continue;
-            if (any_bad) {
-                unsigned bad = 0;
-                for (int w = 0; w < kWarps; ++w) bad |= odd_rows[pair_parity * kWarps + w];
-                if (bad >> tok & 1) {
-                    const int64_t brow = (int64_t)cw.expert * p.n + col;
-                    sum = plain_output(X + (int64_t)(first_row + tok) * p.ldx, p.B + brow * (p.k / 2), scales + brow * p.groups, p.k, 1 << p.group_shift);
-                }
-            }
             out[(int64_t)(first_row + tok) * p.ldo + col] = from_float<T>(sum);
         }
     };
