@@ -289,7 +289,7 @@ typedef enum qm_type {
  *   scale of its row of B, so that a group whose scale is below 2^-14 of that loses digits).
  * So the last place of a row's result can depend on how many rows the call has.  A scale
  * that is not finite makes its column not finite; QM_TYPE_BF16 counts scales from 2^126 on among them.  out is fully overwritten;
- * k == 0 zeroes it, k is at most 2^30 - 32.  n * experts is below 2^31 - 512.  out shares no element with the inputs, here and below.
+ * k == 0 zeroes it, k is at most 2^30 - 32.  m (rows) and n * experts are at most 2^31 - 513.  out shares no element with the inputs, here and below.
  *   k % 32 == 0, ldx % 8 == 0 and 16-byte-aligned X and B need no workspace.  Otherwise X and B are copied into one (device
  *   memory, 16-byte aligned) with k rounded up to 32; qm_gemm_w4_workspace_bytes says how many bytes (experts = 1 for qm_gemm_w4),
  *   QM_ERR_WORKSPACE if there are fewer.
@@ -329,7 +329,8 @@ int qm_quantize_w4(const void *W, int type, int64_t ldw, void *packed, void *sca
  *   xs[slots[t][j]] = X[t]   (`hidden` elements of any qm_type_t; xs holds tokens x top_k rows with pitch ldxs; rows from
  *                offsets[experts] on are left as they were).
  * Many assignments need a workspace (device memory, 4-byte aligned; qm_moe_sort_workspace_bytes says how much, 0 = none,
- * QM_ERR_WORKSPACE if it is smaller).  experts and top_k are at most 4096.
+ * QM_ERR_WORKSPACE if it is smaller).  experts and top_k are at most 4096, tokens * top_k is below 2^31; here and below hidden is at most
+ * 2^31 - 4097.
  */
 int qm_moe_sort(const void *X, int type, int64_t ldx, const void *ids, int id_bytes, int experts, void *xs, int64_t ldxs, int *offsets,
                 int *slots, int tokens, int top_k, int hidden, void *workspace, size_t workspace_bytes, void *stream);

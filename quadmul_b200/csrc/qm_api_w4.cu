@@ -10,13 +10,16 @@ namespace {
 
 constexpr int kMaxK = (1 << 30) - 32;  // a row of X is below 2^31 bytes, rounded up to 32 elements or not
 
+constexpr int kMaxRows = INT_MAX - 512;     // rounded up to whole tiles, and a tile further, it is an int
+constexpr int kMaxHidden = INT_MAX - 4096;  // as is a place in a row, one turn of a block further
+
 bool known_group(int g) { return g == 32 || g == 64 || g == 128 || g == 256; }
 
 bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 int check_w4(const W4Args &a)
 {
-    if (a.rows < 0 || a.n < 0 || a.k < 0 || (a.k & 1) || a.k > kMaxK || a.experts < 0 || a.experts > kMaxExperts) return QM_ERR_SHAPE;
+    if (a.rows < 0 || a.rows > kMaxRows || a.n < 0 || a.k < 0 || (a.k & 1) || a.k > kMaxK || a.experts < 0 || a.experts > kMaxExperts) return QM_ERR_SHAPE;
     if (a.type != QM_TYPE_F16 && a.type != QM_TYPE_BF16) return QM_ERR_ARG;
     if (a.scale_type != QM_TYPE_F32 && a.scale_type != a.type) return QM_ERR_ARG;
     if (!known_group(a.group)) return QM_ERR_ARG;
@@ -46,7 +49,7 @@ int w4_dispatch(W4Args a, void *workspace, size_t workspace_bytes)
 
 int check_moe(int type, int tokens, int top_k, int hidden)
 {
-    if (tokens < 0 || top_k < 0 || top_k > kMaxExperts || hidden < 0 || (int64_t)tokens * top_k > INT_MAX) return QM_ERR_SHAPE;
+    if (tokens < 0 || top_k < 0 || top_k > kMaxExperts || hidden < 0 || hidden > kMaxHidden || (int64_t)tokens * top_k > INT_MAX) return QM_ERR_SHAPE;
     return w4::known_type(type) ? QM_OK : QM_ERR_ARG;
 }
 

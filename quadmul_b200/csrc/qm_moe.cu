@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
     constexpr int kCols = VEC == 1 ? 4 : 1;  // pieces of a row per thread and turn: single elements need more of them in flight
     const int64_t t = blockIdx.x / parts;
     const int part = (int)(blockIdx.x % parts);
-    for (int c0 = (part * kThreads * kCols + (int)threadIdx.x) * VEC; c0 < hidden; c0 += parts * kThreads * kCols * VEC) {
+    // (unsigned: from the last piece of a long row one step goes beyond 2^31)
+    const unsigned width = (unsigned)hidden;
+    for (unsigned c0 = (part * kThreads * kCols + threadIdx.x) * VEC; c0 < width; c0 += (unsigned)parts * (kThreads * kCols * VEC)) {
         float sum[kCols][VEC];
 #pragma unroll
         for (int o = 0; o < kCols; ++o)
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
                 w[j] = weights ? to_float(__ldg(weights + t * top_k + j0 + j)) : 1.0f;
 #pragma unroll
                 for (int o = 0; o < kCols; ++o)
-                    if (c0 + o * kThreads * VEC < hidden) v[j][o].load(ys + (int64_t)at * ldys + c0 + o * kThreads * VEC);
+                    if (c0 + o * kThreads * VEC < width) v[j][o].load(ys + (int64_t)at * ldys + c0 + o * kThreads * VEC);
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
         }
 #pragma unroll
         for (int o = 0; o < kCols; ++o) {
-            if (c0 + o * kThreads * VEC >= hidden) continue;
+            if (c0 + o * kThreads * VEC >= width) continue;
             Piece<T, VEC> r;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) r.v[i] = from_float<T>(sum[o][i]);
@@ -329,10 +331,12 @@ int with_pieces(bool vec, F f)
 
 constexpr int kMaxSlots = 8192;  // slots a block keeps in shared memory; top_k is at most half of it
 
+int block_count(int tokens, int per) { return (int)(((int64_t)tokens + per - 1) / per); }
+
 int tokens_per_block(int tokens, int top_k)
 {
     const int blocks = (int64_t)tokens * top_k <= kFewIds ? kFewBlocks : kManyBlocks;
-    const int per = (tokens + blocks - 1) / blocks, most = kMaxSlots / (top_k > 0 ? top_k : 1);
+    const int per = (int)(((int64_t)tokens + blocks - 1) / blocks), most = kMaxSlots / (top_k > 0 ? top_k : 1);
     return per < 1 ? 1 : per < most ? per : most;
 }
 
@@ -341,13 +345,13 @@ int tokens_per_block(int tokens, int top_k)
 size_t moe_sort_workspace(int tokens, int top_k, int experts)
 {
     if ((int64_t)tokens * top_k <= kFewIds) return 0;
-    const int per = tokens_per_block(tokens, top_k), blocks = (tokens + per - 1) / per;
+    const int blocks = block_count(tokens, tokens_per_block(tokens, top_k));
     return ((size_t)blocks + 1) * experts * sizeof(int);
 }
 
 int moe_sort_launch(const MoeSortArgs &a)
 {
-    const int per = tokens_per_block(a.tokens, a.top_k), blocks = a.tokens > 0 ? (a.tokens + per - 1) / per : 1;
+    const int per = tokens_per_block(a.tokens, a.top_k), blocks = a.tokens > 0 ? block_count(a.tokens, per) : 1;
     const int count = a.tokens * a.top_k;
     const size_t smem = ((size_t)2 * a.experts + (size_t)per * a.top_k) * sizeof(int);
     int *counts = nullptr, *totals = nullptr;
