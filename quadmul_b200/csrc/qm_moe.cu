@@ -14,6 +14,8 @@
 // Measured (bf16): sort of 16 x 8 by 64 experts 5.9 us, of 8192 x 2 rows of 4096 45 us = 4.5 TB/s; combine of 4096 x 8 rows of
 // 4096 47 us = 6.4 TB/s, its gradients 90 us = 6.4 TB/s (0.97 of a copy).  Single elements (rows off 16-byte boundaries, 3000 x 4 of
 // 5119): sort 66 us = 2.3 TB/s, combine 49 us = 3.1.
+#include <atomic>
+
 #include "qm_w4.cuh"
 
 namespace qm {
@@ -331,6 +333,8 @@ int with_pieces(bool vec, F f)
 
 constexpr int kMaxSlots = 8192;  // slots a block keeps in shared memory; top_k is at most half of it
 
+constexpr size_t kMaxSmem = (2 * (size_t)kMaxExperts + kMaxSlots) * sizeof(int);
+
 int block_count(int tokens, int per) { return (int)(((int64_t)tokens + per - 1) / per); }
 
 int tokens_per_block(int tokens, int top_k)
@@ -375,8 +379,17 @@ int moe_sort_launch(const MoeSortArgs &a)
                 constexpr int VEC = decltype(v)::value;
                 auto kernel = moe_place_kernel<T, I, VEC>;
                 if (smem > 48 * 1024) {
-                    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                    if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(moe_place_kernel)");
+                    // The limit belongs to the kernel, not to the launch: the largest one, set once per device, so that no call can lower
+                    // it between another thread's setting and its launch (a repeated cudaFuncSetAttribute is harmless).
+                    static std::atomic<bool> configured[64];
+                    int device = 0;
+                    cudaError_t e = cudaGetDevice(&device);
+                    if (e != cudaSuccess) return record_cuda_error(e, "cudaGetDevice");
+                    if (!configured[device & 63].load(std::memory_order_acquire)) {
+                        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+                        if (e != cudaSuccess) return record_cuda_error(e, "cudaFuncSetAttribute(moe_place_kernel)");
+                        configured[device & 63].store(true, std::memory_order_release);
+                    }
                 }
                 return launch_in_turn("moe_place_kernel launch", kernel, (unsigned)blocks, kSortThreads, smem, a.stream, static_cast<const T *>(a.X), a.ldx, ids,
                                       a.experts, a.tokens, a.top_k, a.hidden, per, (const int *)counts, (const int *)totals, static_cast<T *>(a.xs), a.ldxs,
