@@ -12,15 +12,22 @@ from __future__ import annotations
 
 from . import _EXT, _count, _on_device, _stream_of, _torch
 from ._lib import LIB, check
-from .w4 import check_out, check_rows, check_whole, compiled, moe_gemm_w4, pitch, type_of
+from .w4 import check_out, check_rows, check_sizes, check_whole, compiled, moe_gemm_w4, pitch, type_of
 
 MAX_EXPERTS = 4096
+
+
+def check_assignments(what, tokens, top_k):
+    check_sizes(what, "the number of tokens", (tokens,))
+    if top_k > MAX_EXPERTS or tokens * top_k >= 1 << 31:
+        raise ValueError(f"{what}: too many assignments")
 
 
 def _check_slots(what, slots, device):
     if slots.dim() != 2 or slots.dtype != _torch().int32:
         raise ValueError(f"{what}: slots must be int32 [tokens, top_k]")
     check_whole(what, device, slots=slots)
+    check_assignments(what, *slots.shape)
 
 
 def _check_weights(what, weights, slots, like):
@@ -56,8 +63,7 @@ def moe_sort(x, expert_ids, num_experts: int, out=None):
     if not 0 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"{what}: num_experts must be within [0, {MAX_EXPERTS}]")
     (tokens, hidden), top_k = x.shape, expert_ids.shape[1]
-    if top_k > MAX_EXPERTS or tokens * top_k >= 1 << 31:
-        raise ValueError(f"{what}: too many assignments")
+    check_assignments(what, tokens, top_k)
     xs = check_out(what, "out", out, (tokens * top_k, hidden), x)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=x.device)
     slots = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)

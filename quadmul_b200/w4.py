@@ -35,6 +35,12 @@ def type_of(what: str, name: str, t, allowed=None) -> int:
     return code
 
 
+def check_sizes(what: str, name: str, shape) -> None:
+    """The library takes sizes as 32-bit ints, and ctypes would drop what is above them."""
+    if any(size >= 1 << 31 for size in shape):
+        raise ValueError(f"{what}: {name} is too large")
+
+
 def check_rows(what: str, **tensors) -> None:
     """2-D CUDA tensors of one device whose rows are contiguous; none that autograd would have to record."""
     torch = _torch()
@@ -49,6 +55,7 @@ def check_rows(what: str, **tensors) -> None:
             raise ValueError(f"{what}: {name} must have two dimensions")
         if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
             raise ValueError(f"{what}: the rows of {name} must be contiguous and must not overlap")
+        check_sizes(what, name, t.shape)
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what}: {name} requires a gradient, which this call does not record")
 
@@ -106,6 +113,7 @@ def _check_weights(what, x, b, scales, group, lead):
         raise ValueError(f"{what}: k must be even")
     if b.dim() != 2 + len(lead) or tuple(b.shape[:-2]) != lead or b.shape[-1] != k // 2:
         raise ValueError(f"{what}: b has shape {tuple(b.shape)}, x has {k} columns")
+    check_sizes(what, "b", b.shape)
     n = b.shape[-2]
     if tuple(scales.shape) != (*lead, n, -(-k // group)):
         raise ValueError(f"{what}: scales have shape {tuple(scales.shape)}, expected {(*lead, n, -(-k // group))}")
