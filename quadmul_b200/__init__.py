@@ -46,7 +46,7 @@ __all__ = [
     "moe_linear_w4",
 ]
 
-_launches = 0  # kernels this package launched (one per call below; split-K adds none)
+_launches = 0  # kernels this package launched (one per call below; split-K adds none); the compiled binding counts its own
 
 # The compiled binding (csrc/torch_binding.cpp, built by `python -m quadmul_b200.build --torch`) shortens the host side
 # of gemm(); without it the same C-ABI entry point is reached through ctypes.  Either way the work is qm_gemm_s4.
@@ -57,7 +57,8 @@ except Exception:  # not built, or built against another torch
 
 
 def launch_count() -> int:
-    return _launches
+    """Kernels that this package has launched: refused calls and calls with nothing to do add none."""
+    return _launches + (_EXT.launched() if _EXT is not None else 0)
 
 
 def _count(launches: int) -> None:

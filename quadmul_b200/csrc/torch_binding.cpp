@@ -40,6 +40,9 @@ void gemm(torch::Tensor a, torch::Tensor b, torch::Tensor c, int64_t m, int64_t 
     TORCH_CHECK(st == QM_OK, "quadmul.gemm(m=", m, ", n=", n, ", k=", k, "): ", qm_status_string(st), " ", qm_last_cuda_error());
 }
 
+// Kernels that the calls below have launched (the interpreter's lock is held: they run one at a time)
+int64_t launched = 0;
+
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 
@@ -134,6 +137,15 @@ Tensor workspace_for(const Tensor &x, const Tensor &b, int64_t experts, const We
     return need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
 }
 
+// The product's kernel and the copies in front of it
+int64_t product_launches(const Tensor &x, const Tensor &b, int64_t experts, const Weights &w)
+{
+    if (x.size(0) == 0 || w.n == 0 || experts == 0) return 0;
+    if (w.k == 0) return 1;
+    auto off = [&](const Tensor &t) { return w.k % 32 != 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0; };
+    return 1 + (off(x) || pitch(x) % 8 != 0) + off(b);
+}
+
 Tensor gemm_w4(const Tensor &x, const Tensor &b, const Tensor &scales, int64_t group, const OptTensor &out)
 {
     const char *what = "gemm_w4";
@@ -144,6 +156,7 @@ Tensor gemm_w4(const Tensor &x, const Tensor &b, const Tensor &scales, int64_t g
     check_status(what, qm_gemm_w4(x.data_ptr(), w.type, pitch(x), b.data_ptr(), scales.data_ptr(), w.scale_type, (int)group, y.data_ptr(), pitch(y),
                                   (int)x.size(0), (int)w.n, (int)w.k, space.defined() ? space.data_ptr() : nullptr,
                                   space.defined() ? space.numel() : 0, stream_of(x)));
+    launched += product_launches(x, b, 1, w);
     return y;
 }
 
@@ -161,6 +174,7 @@ Tensor moe_gemm_w4(const Tensor &x, const Tensor &b, const Tensor &scales, const
     check_status(what, qm_moe_gemm_w4(x.data_ptr(), w.type, pitch(x), b.data_ptr(), scales.data_ptr(), w.scale_type, (int)group,
                                       static_cast<const int *>(offsets.data_ptr()), (int)b.size(0), y.data_ptr(), pitch(y), (int)x.size(0), (int)w.n,
                                       (int)w.k, space.defined() ? space.data_ptr() : nullptr, space.defined() ? space.numel() : 0, stream_of(x)));
+    launched += product_launches(x, b, b.size(0), w);
     return y;
 }
 
@@ -178,6 +192,7 @@ std::tuple<Tensor, Tensor> quantize_w4(const Tensor &w, int64_t group, bool floa
     c10::cuda::CUDAGuard guard(w.device());
     check_status(what, qm_quantize_w4(w.data_ptr(), type, pitch(w), packed.data_ptr(), scales.data_ptr(), float_scales ? QM_TYPE_F32 : type, n, k,
                                       (int)group, stream_of(w)));
+    launched += n > 0 && k > 0;
     return {packed, scales};
 }
 
@@ -203,6 +218,7 @@ std::tuple<Tensor, Tensor, Tensor> moe_sort(const Tensor &x, const Tensor &ids, 
     check_status(what, qm_moe_sort(x.data_ptr(), type, pitch(x), ids.data_ptr(), (int)ids.element_size(), (int)experts, xs.data_ptr(), pitch(xs),
                                    static_cast<int *>(offsets.data_ptr()), static_cast<int *>(slots.data_ptr()), (int)tokens, (int)top_k, (int)hidden,
                                    need ? workspace.data_ptr() : nullptr, need, stream_of(x)));
+    launched += need ? 3 : 1;
     return {xs, offsets, slots};
 }
 
@@ -234,6 +250,7 @@ Tensor moe_combine(const Tensor &ys, const Tensor &slots, const OptTensor &weigh
     check_status(what, qm_moe_combine(ys.data_ptr(), type, pitch(ys), (int)ys.size(0), static_cast<const int *>(slots.data_ptr()),
                                       weights ? weights->data_ptr() : nullptr, weight_type, y.data_ptr(), pitch(y), (int)slots.size(0), (int)slots.size(1),
                                       (int)ys.size(1), stream_of(ys)));
+    launched += y.numel() > 0;
     return y;
 }
 
@@ -253,6 +270,7 @@ std::tuple<Tensor, Tensor> moe_combine_grad(const Tensor &dy, const Tensor &ys, 
     check_status(what, qm_moe_combine_grad(dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys), type, (int)ys.size(0), static_cast<const int *>(slots.data_ptr()),
                                            weights.data_ptr(), weight_type, dys.data_ptr(), pitch(dys), dweights.data_ptr(), (int)slots.size(0),
                                            (int)slots.size(1), (int)ys.size(1), stream_of(ys)));
+    launched += dweights.numel() > 0;
     return {dys, dweights};
 }
 
@@ -267,4 +285,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod)
     mod.def("moe_sort", &moe_sort, "rows in expert order, offsets, slots");
     mod.def("moe_combine", &moe_combine, "weighted sum of the experts' rows per token");
     mod.def("moe_combine_grad", &moe_combine_grad, "gradients of moe_combine");
+    mod.def("launched", [] { return launched; }, "kernels that the calls other than gemm have launched");
 }

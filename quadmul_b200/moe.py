@@ -50,9 +50,7 @@ def moe_sort(x, expert_ids, num_experts: int, out=None):
     what = "moe_sort"
     torch = _torch()
     if _EXT is not None:
-        result = compiled(_EXT.moe_sort, x, expert_ids, num_experts, out)
-        _count(3 if LIB.qm_moe_sort_workspace_bytes(*expert_ids.shape, num_experts) else 1)
-        return result
+        return compiled(_EXT.moe_sort, x, expert_ids, num_experts, out)
     code = type_of(what, "x", x)
     check_rows(what, x=x)
     check_whole(what, x.device, expert_ids=expert_ids)
@@ -85,7 +83,6 @@ def moe_combine(ys, slots, weights=None, out=None):
     without any gets zeros); weights [tokens, top_k] of ys's type or float32, None for all ones."""
     what = "moe_combine"
     if _EXT is not None:
-        _count(1)
         return compiled(_EXT.moe_combine, ys, slots, weights, out)
     code = type_of(what, "ys", ys)
     check_rows(what, ys=ys)
@@ -97,7 +94,7 @@ def moe_combine(ys, slots, weights=None, out=None):
         st = LIB.qm_moe_combine(ys.data_ptr(), code, pitch(ys), rows, slots.data_ptr(), None if weights is None else weights.data_ptr(), wcode,
                                 y.data_ptr(), pitch(y), tokens, top_k, hidden, _stream_of(ys))
     check(st, f"{what}(tokens={tokens}, top_k={top_k}, hidden={hidden}, rows={rows})")
-    _count(1)
+    _count(int(y.numel() > 0))
     return y
 
 
@@ -114,7 +111,6 @@ def moe_combine_grad(dy, ys, slots, weights, out=None):
     as they were in `out` (and undefined in a dys that is allocated here)."""
     what = "moe_combine_grad"
     if _EXT is not None:
-        _count(1)
         return compiled(_EXT.moe_combine_grad, dy, ys, slots, weights, out)
     torch = _torch()
     code = type_of(what, "dy", dy)
@@ -132,7 +128,7 @@ def moe_combine_grad(dy, ys, slots, weights, out=None):
         st = LIB.qm_moe_combine_grad(dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys), code, rows, slots.data_ptr(), weights.data_ptr(), wcode,
                                      dys.data_ptr(), pitch(dys), dweights.data_ptr(), tokens, top_k, hidden, _stream_of(ys))
     check(st, f"{what}(tokens={tokens}, top_k={top_k}, hidden={hidden}, rows={rows})")
-    _count(1)
+    _count(int(dweights.numel() > 0))
     return dys, dweights
 
 

@@ -86,6 +86,16 @@ def _workspace(x, b, experts, n):
     return space, space.data_ptr(), need
 
 
+def _product_launches(x, b, experts, n) -> int:
+    """The product's kernel and the copies in front of it."""
+    (rows, k) = x.shape
+    if not (rows and n and experts):
+        return 0
+    if not k:
+        return 1
+    return 1 + bool(k % 32 or pitch(x) % 8 or x.data_ptr() % 16) + bool(k % 32 or b.data_ptr() % 16)
+
+
 def check_out(what: str, name: str, out, shape, like):
     torch = _torch()
     if out is None:
@@ -132,7 +142,6 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
     current stream of x's device."""
     what = "gemm_w4"
     if _EXT is not None:
-        _count(1)
         return compiled(_EXT.gemm_w4, x, b, scales, group, out)
     code, scode, n, k = _check_weights(what, x, b, scales, group, ())
     m = x.shape[0]
@@ -142,7 +151,7 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
         st = LIB.qm_gemm_w4(x.data_ptr(), code, pitch(x), b.data_ptr(), scales.data_ptr(), scode, group, out.data_ptr(), pitch(out), m, n, k, ptr,
                             size, _stream_of(x))
     check(st, f"{what}(m={m}, n={n}, k={k}, group={group})")
-    _count(1)
+    _count(_product_launches(x, b, 1, n))
     return out
 
 
@@ -154,7 +163,6 @@ def moe_gemm_w4(x, b, scales, offsets, group: int = 128, out=None):
     undefined in an `out` that is allocated here).  The launch does not depend on the values of offsets."""
     what = "moe_gemm_w4"
     if _EXT is not None:
-        _count(1)
         return compiled(_EXT.moe_gemm_w4, x, b, scales, offsets, group, out)
     torch = _torch()
     if b.dim() != 3:
@@ -171,7 +179,7 @@ def moe_gemm_w4(x, b, scales, offsets, group: int = 128, out=None):
         st = LIB.qm_moe_gemm_w4(x.data_ptr(), code, pitch(x), b.data_ptr(), scales.data_ptr(), scode, group, offsets.data_ptr(), experts,
                                 out.data_ptr(), pitch(out), rows, n, k, ptr, size, _stream_of(x))
     check(st, f"{what}(rows={rows}, n={n}, k={k}, experts={experts}, group={group})")
-    _count(1)
+    _count(_product_launches(x, b, experts, n))
     return out
 
 
@@ -187,7 +195,6 @@ def quantize_w4(w, group: int = 128, scale_dtype=None):
     if scale_dtype not in (w.dtype, torch.float32):
         raise TypeError(f"{what}: scale_dtype must be {w.dtype} or torch.float32")
     if _EXT is not None:
-        _count(1)
         return compiled(_EXT.quantize_w4, w, group, scale_dtype == torch.float32)
     code = type_of(what, "w", w)
     check_rows(what, w=w)
@@ -202,5 +209,5 @@ def quantize_w4(w, group: int = 128, scale_dtype=None):
         st = LIB.qm_quantize_w4(w.data_ptr(), code, pitch(w), packed.data_ptr(), scales.data_ptr(), type_of(what, "scales", scales), n, k, group,
                                 _stream_of(w))
     check(st, f"{what}(n={n}, k={k}, group={group})")
-    _count(1)
+    _count(int(n > 0 and k > 0))
     return packed, scales
