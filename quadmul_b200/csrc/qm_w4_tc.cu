@@ -695,7 +695,7 @@ int max_clusters(int device, int size)
     cfg.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, w4_tc_kernel<G, T, S>, &cfg) != cudaSuccess || n < 1) {
         (void)cudaGetLastError();
-        n = 1;
+        return 1;  // right, if slow, and asked again next time
     }
     slot.store(n, std::memory_order_relaxed);
     return n;
