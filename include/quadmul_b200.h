@@ -282,7 +282,7 @@ typedef enum qm_type {
  * X (m x k, row pitch ldx elements) times the transpose of B into out (m x n, row pitch ldo elements); X and out are both
  * QM_TYPE_F16 or both QM_TYPE_BF16 (`type`), the scales have that type or QM_TYPE_F32, group is 32, 64, 128 or 256, k is even.
  * Sums are fp32 and are rounded to `type` once.  Beside that an element or a weight is rounded, by the number of rows:
- *   up to 8 rows (on average per expert), where they fit the kernel for few rows: X is read to 22 bits below the largest of its (at
+ *   up to 8 rows (experts: 6 on average), where they fit the kernel for few rows: X is read to 22 bits below the largest of its (at
  *   most 128) neighbours under one scale; a row in which more than a quarter of the elements of such a stretch would lose digits is
  *   summed in fp32 as it is.
  *   otherwise: a weight scale * q is rounded to `type` before it is multiplied, by at most half a step (fp16: relative to the largest

@@ -43,7 +43,11 @@ int w4_dispatch(W4Args a, void *workspace, size_t workspace_bytes)
     if (a.k == 0) return w4_zero_launch(a);
     if (need && (st = w4_pad_launch(&a, workspace)) != QM_OK) return st;
     const int average = a.rows / (a.experts < a.rows ? a.experts : a.rows);
-    if (average <= 8 && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
+    // The kernel for few rows up to a whole pass over the weights.  One matrix, rows against tcgen05 kernel: 8 x 4096 x 4096 8.2 and 10.3
+    // us, 9 rows (two passes) 10.9 and 10.3; 8 x 11008 x 4096 13.8 and 17.2, 9 rows 20.2 and 17.5.  With experts some have more rows
+    // than the average, and theirs are two passes: 32 experts of 4096 x 4096 with 6 rows on average 81 and 92 us, with 8 100 and 92;
+    // 8 of 11008 x 4096 60 and 67, 70 and 67; 64 of 1024 x 2048 36 and 35, 43 and 35.
+    if (average <= (a.offsets ? 6 : 8) && w4_rows_eligible(a, *ctx)) return w4_rows_launch(a, *ctx);
     return w4_tc_launch(a, *ctx);
 }
 

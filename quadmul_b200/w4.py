@@ -135,7 +135,7 @@ def gemm_w4(x, b, scales, group: int = 128, out=None):
 
     x: float16 or bfloat16, rows contiguous (a column slab of a wider tensor is fine); b: packed codes [n, k/2] as `pack` and
     `quantize_w4` write them; scales [n, ceil(k / group)]: x's type or float32; group: 32, 64, 128 or 256.  Returns out, of x's
-    type (allocated when not passed in).  Sums are fp32.  With up to 8 rows x is read to 22 bits below the largest of its neighbours
+    type (allocated when not passed in).  Sums are fp32.  With up to 8 rows (experts: 6 on average) x is read to 22 bits below the largest of its neighbours
     under one scale (a row that would lose more than a few elements' digits by that is summed as it is); with more rows, or where 8
     rows of k elements do not fit the kernel for few rows, a weight is rounded to x's type before it is multiplied.
     k a multiple of 32 and rows of x and b on 16-byte boundaries are fastest: others are copied first.  Asynchronous on the
