@@ -1,6 +1,6 @@
 // Tokens to experts and back: a stable counting sort of the assignments with the copy of their rows, the weighted sum that
 // brings the experts' rows back, and the gradients of both.  All of it is bound by memory: rows move in 16-byte pieces with
-// several in flight per thread, and nothing is read twice but indices.
+// several in flight per thread, and nothing is read twice but indices (and dy, for every four of top_k).
 //
 // Sorting.  slot(t, j) = (assignments to lower experts) + (earlier assignments to the same expert): a counting sort, stable, without
 // atomics on anything that decides an order.  Up to kFewIds assignments take ONE launch: every block counts all ids itself
@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(const T *__restri
     }
 }
 
-// Both gradients of one token: dy is read once, every row of ys once, every row of dys is written once; the products with the
-// rows are summed over the block in a fixed order.
+// Both gradients of one token: dy is read once for every four of its experts, every row of ys once, every row of dys is written once;
+// the products with the rows are summed over the block in a fixed order.
 template <typename T, typename S, int VEC>
 __global__ void __launch_bounds__(kThreads) moe_combine_grad_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ ys, int64_t ldys, int rows,
                                                                     const int *__restrict__ slots, const S *__restrict__ weights, T *__restrict__ dys,
