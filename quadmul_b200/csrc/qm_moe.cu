@@ -11,8 +11,8 @@
 // The launches take their turn in the stream: these kernels read indices that the kernel before may have written, and addresses come
 // from them, so none starts before that one has ended.
 //
-// Measured (bf16): sort of 16 x 8 by 64 experts 5.9 us, of 8192 x 2 rows of 4096 45 us = 4.5 TB/s; combine of 4096 x 8 rows of
-// 4096 47 us = 6.4 TB/s, its gradients 90 us = 6.4 TB/s (0.97 of a copy).  Single elements (rows off 16-byte boundaries, 3000 x 4 of
+// Measured (bf16): sort of 16 x 8 by 64 experts 8.2 us, of 8192 x 2 rows of 4096 48.6 us = 4.1 TB/s; combine of 4096 x 8 rows of
+// 4096 49 us = 6.1 TB/s, its gradients 93 us = 6.1 TB/s (0.93 of a copy).  Single elements (rows off 16-byte boundaries, 3000 x 4 of
 // 5119): sort 66 us = 2.3 TB/s, combine 49 us = 3.1.
 #include <atomic>
 

@@ -1,12 +1,14 @@
 // Group-wise 4-bit quantiser: per group of a row, scale = max |w| times the fp32 value of 1/7 (rounded to the scales' type) and
 // code = w / scale, the exact quotient rounded to the nearest integer, ties to even.
 //
-// Every element is read once and leaves as half a byte, so memory should bound it; what it costs beside that is arithmetic.  A lane
+// Every element is read once and leaves as half a byte, so memory should bound it, as it does for fp32.  With 16-bit elements
+// there are twice as many to convert per byte, and a warp's loads and conversions take turns: 11008 x 4096 bf16 keeps DRAM at 38 % and
+// the SM at 66 % of their peaks.  A lane
 // takes sixteen consecutive elements (two or four 16-byte loads) and writes their eight bytes; 2, 4, 8 or 16 neighbouring lanes
 // share a group, whose maximum is a few shuffles.  A warp has kUnroll such pieces of 512 elements in flight.
 //
-// Measured: 22016 x 4096 fp32 in groups of 32 65.7 us = 6.35 TB/s (0.97 of a copy); 4096 x 4096 bf16 in groups of 128 12.6 us =
-// 3.4 TB/s, bound by the arithmetic.  Any alignment: 11008 x 4094 bf16 108 us.
+// Measured: 22016 x 4096 fp32 in groups of 32 64 us = 6.5 TB/s (0.99 of a copy); bf16 in groups of 128 14.4 us for 4096 x 4096 = 2.9
+// TB/s, 30 us for 11008 x 4096 = 3.8.  Any alignment: 11008 x 4094 bf16 109 us.
 #include <type_traits>
 
 #include "qm_w4.cuh"

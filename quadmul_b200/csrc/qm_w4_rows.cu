@@ -30,9 +30,9 @@
 //    Otherwise (1 or 2 rows) the three bytes of both rows take six columns of one instruction.
 //  * The warps' partial tiles meet in shared memory (two buffers, one barrier a block) and are added in a fixed order.
 //
-// Measured (groups of 128, bf16): 1 x 57344 x 8192 54 us = 4.45 TB/s, 8 rows of it 87 us; 1 x 4096 x 4096 5.2 us, of which a launch
-// in a dependent chain is 2.4; 128 rows over 32 experts of 4096 x 4096 72 us = 3.9 TB/s, DRAM at 47 % and the s8 pipe at 36 % of
-// their peaks.  Groups of 32 cost 1.3 us more at 1 x 4096 x 4096: the lanes trade words.
+// Measured (groups of 128, bf16): 1 x 57344 x 8192 53.4 us = 4.5 TB/s, 8 rows of it 89 us; 1 x 4096 x 4096 4.9 us, of which a launch
+// in a dependent chain is 2.4; 128 rows over 32 experts of 4096 x 4096 73-77 us = 3.6-3.8 TB/s, DRAM at 45 % and the SM at 43 % of
+// their peaks.  Groups of 32 cost 1.2 us more at 1 x 4096 x 4096: the lanes trade words.
 //
 // With experts a unit of work is (expert, tile of its rows, block of B); every CTA takes a contiguous range of units, so the rows
 // of X change rarely.
@@ -563,8 +563,9 @@ bool rows_plan(const W4Args &a, int sms, RowsPlan *plan)
     const int steps = (a.k + kStep - 1) / kStep;
     p.wide = a.offsets ? a.rows > (a.experts < a.rows ? a.experts : a.rows) : a.rows > kNarrowRows;
     // Warps that split K: all, or as many as there are steps.  Only where a CTA has many blocks to do, and the block's end is long (WIDE),
-    // warp groups that take turns at it pay: 4096 units over 148 CTAs (27 each), 8 rows, 4096 x 4096: 84 us with WK = 16, 71 with 4;
-    // 896 units (6 each): 35.0 against 37.4; 1792 units of one row: 55.6 against 64.7.
+    // warp groups that take turns at it pay (us with WK = 16, 8 and 4): 128 rows over 32 experts of 4096 x 4096, at most 28 units a CTA,
+    // 84, 78 and 78; 8 x 57344 x 8192, 12 units, 90, 88 and 112; 8 x 28672 x 4096, 6 units, 24.2, 25.1 and 25.4; one row of
+    // 57344 x 8192 53.7, 55.0 and 59.0.  (8 is within 4 % of the better of the two on either side.)
     const int tile = p.wide ? kWideRows : kNarrowRows;
     const int64_t pairs = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : (a.rows + tile - 1) / tile;  // (with experts: at most)
     const int64_t units = pairs * ((a.n + kRows - 1) / kRows);

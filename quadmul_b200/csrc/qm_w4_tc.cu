@@ -24,11 +24,11 @@
 // part of K; the partial tiles meet in the CTAs' shared memory and are added in a fixed order.
 // All waits are bounded as in gemm_tc_kernel.
 //
-// Measured (groups of 128, bf16): 2048 x 12288 x 4096 143 us = 1.44 PFLOP/s, tensor pipe 82 % active (fp16 150 us; the library's
-// 16-bit product of that size 135); 8192 rows over 8 experts of 11008 x 4096 545 us = 1.36 PFLOP/s.  Few columns per item are bound by
-// the stages' turn-round, about 700 clocks each: 512 rows over 32 experts of 4096 x 4096 96 us = 2.9 TB/s; a quarter of the MMAs, no
-// tcgen05.st, longer rings or wider loads change that by 3 % at most, no conversion by 14 %.  SPLIT is a chain of latencies:
-// 16 x 4096 x 4096 9.8 us, 128 x 4096 x 4096 12.8.
+// Measured (groups of 128, bf16, a few calls in a row; a long run meets the power cap): 2048 x 12288 x 4096 138-142 us = 1.45-1.49
+// PFLOP/s, tensor pipe 82 % active (fp16 144-149 us; the library's 16-bit product of that size 136); 8192 rows over 8 experts of 11008 x
+// 4096 505 us = 1.46 PFLOP/s (fp16 529).  Few columns per item are bound by the stages' turn-round, about 700 clocks each: 512 rows
+// over 32 experts of 4096 x 4096 95 us = 2.9 TB/s; a quarter of the MMAs, no tcgen05.st, longer rings or wider loads change that by
+// 3 % at most, no conversion by 14 %.  SPLIT is a chain of latencies: 16 x 4096 x 4096 10.2 us, 128 x 4096 x 4096 13.2.
 #include <cuda.h>
 
 #include <atomic>
