@@ -13,8 +13,9 @@
 //   That is nothing beside the other elements' products, but a weight of zero can take the largest one out of a sum.  So where more
 //   than a quarter of a stretch's elements lose digits (an element hundreds, fp16, or thousands of times its neighbours), or one is an
 //   infinity or a NaN, the row's outputs are computed from their definition instead, element by element: 1 x 4096 x 4096 14 us,
-//   8 x 4096 x 4096 58 us with all rows so.  Finding out costs a vote per 256 elements of X, and a count (8 x 4096 x 4096 8.2 -> 10.2
-//   us) only where eight neighbours have nothing above 2^-8 of their stretch's largest.
+//   8 x 4096 x 4096 58 us with all rows so.  Finding out costs a vote per 256 elements of X, and a count where one of them is small
+//   enough to lose digits: 8 x 4096 x 4096 of normal numbers 7.8 -> 8.3 us (fp16, whose digits reach further down, 8.9; 10.2 where every
+//   piece is counted).
 //
 //  * A CTA (16 warps) takes blocks of 32 rows of B per warp group; WK of its warps split K between them in steps of 128 elements.
 //    Lane (g, q) = (lane / 4, lane % 4) loads 16 bytes, 32 codes, of row g of each 8-row group straight into registers; kDepth steps
@@ -30,7 +31,7 @@
 //    Otherwise (1 or 2 rows) the three bytes of both rows take six columns of one instruction.
 //  * The warps' partial tiles meet in shared memory (two buffers, one barrier a block) and are added in a fixed order.
 //
-// Measured (groups of 128, bf16): 1 x 57344 x 8192 53.4 us = 4.5 TB/s, 8 rows of it 89 us; 1 x 4096 x 4096 4.9 us, of which a launch
+// Measured (groups of 128, bf16): 1 x 57344 x 8192 53.4 us = 4.5 TB/s, 8 rows of it 90 us; 1 x 4096 x 4096 4.9 us, of which a launch
 // in a dependent chain is 2.4; 128 rows over 32 experts of 4096 x 4096 73-77 us = 3.6-3.8 TB/s, DRAM at 45 % and the SM at 43 % of
 // their peaks.  Groups of 32 cost 1.2 us more at 1 x 4096 x 4096: the lanes trade words.
 //
@@ -186,15 +187,26 @@ __device__ __forceinline__ Stretch stretch_of(uint32_t m)
     return s;
 }
 
-// Whether the stretch that LANES neighbouring lanes have eight elements of each cannot be written as bytes: one is not finite, or more
-// than a quarter of those that are not zero lose digits.  The whole warp.  These are counted only where some lane of it has nothing
-// above 2^-8 of its stretch's largest (m; `here` is the lane's own).
-template <typename T, int LANES>
-__device__ __forceinline__ bool loses_digits(const uint4 &v, uint32_t here, uint32_t m, const Stretch &s)
+// One less than the smallest magnitude of eight elements that is not zero, as the bits of T (0xFFFF: all are zero): with the sign bit
+// set and one taken away a zero is the largest signed number, the others keep their order.
+__device__ __forceinline__ uint32_t smallest_less_one(const uint4 &v)
 {
-    constexpr uint32_t kOctaves = std::is_same<T, __half>::value ? 8u << 10 : 8u << 7;  // in the exponent: a factor of 2^8
+    auto key = [](uint32_t w) { return (w | 0x80008000u) - 0x00010001u; };
+    const uint32_t k = __vmins2(__vmins2(key(v.x), key(v.y)), __vmins2(key(v.z), key(v.w))) ^ 0x80008000u;
+    return min(k & 0xFFFFu, k >> 16);
+}
+
+// Whether the stretch that LANES neighbouring lanes have eight elements of each cannot be written as bytes: one is not finite, or more
+// than a quarter of those that are not zero lose digits.  The whole warp.  These are counted only where some lane of it has one that
+// is so much smaller than its stretch's largest (m) that it can lose some: T's digits end where the 21 bits below m's power of two do.
+template <typename T, int LANES>
+__device__ __forceinline__ bool loses_digits(const uint4 &v, uint32_t m, const Stretch &s)
+{
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr int kMantissa = kHalf ? 10 : 7, kExponent = kHalf ? 0x7C00 : 0x7F80;
     bool bad = s.e == 255u;
-    if (__any_sync(0xFFFFFFFFu, here != 0u && (here + kOctaves < m || s.e < 25u))) {
+    const int exact_from = s.e < 25u ? kExponent : (int)(m & kExponent) - ((20 - kMantissa) << kMantissa);
+    if (__any_sync(0xFFFFFFFFu, (int)smallest_less_one(v) + 1 < exact_from)) {
         int count = 0;  // elements that are not zero, and in the upper half those that lose digits
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -368,12 +380,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const RowsParams p
                 const int row = 2 * r + side;
                 if (2 * r >= tokens) continue;  // (columns without a row hold anything: nobody reads their sums)
                 uint32_t m = magnitudes(v[r]);
-                const uint32_t here = max(m & 0xFFFFu, m >> 16);
 #pragma unroll
                 for (int d = 1; d < 16 / GPS; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
                 m = max(m & 0xFFFFu, m >> 16);
                 const Stretch st = stretch_of<T>(m);
-                if (loses_digits<T, 16 / GPS>(v[r], here, m, st)) bad |= 1u << row;
+                if (loses_digits<T, 16 / GPS>(v[r], m, st)) bad |= 1u << row;
                 uint32_t z[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {

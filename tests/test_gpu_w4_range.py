@@ -108,3 +108,21 @@ def test_equal_calls_give_equal_bits(qm, cuda_clean, m, dtype):
     first = qm.gemm_w4(*args)
     for _ in range(10):
         assert torch.equal(first, qm.gemm_w4(*args))
+
+
+@pytest.mark.parametrize("m", [1, 2, 8])
+@pytest.mark.parametrize("every", [2, 3, 4, 8, 16])
+@pytest.mark.parametrize("dtype,octaves", [(BF16, 22), (FP16, 17)])
+def test_large_elements_at_a_regular_distance(qm, cuda_clean, m, every, dtype, octaves):
+    """One element in `every` is large, and half the columns have code 0 on all of these."""
+    n, k, group = 96, 1024, 128
+    gen = torch.Generator().manual_seed(every)
+    x, q = torch.randn(m, k, generator=gen), codes((n, k), gen)[0]
+    q = torch.where(q == 0, 1, q)
+    x[:, ::every] = 2.0**octaves * (1 + torch.rand(m, x[:, ::every].shape[1], generator=gen))
+    q[: n // 2, ::every] = 0
+    x = (x.double() * 2.0 ** (-2 if dtype == BF16 else -5)).to(dtype)
+    packed = ((q[:, 0::2] & 15) | ((q[:, 1::2] & 15) << 4)).to(torch.uint8).view(torch.int8)
+    scales = (0.01 * torch.exp(0.5 * torch.randn(n, k // group, generator=gen))).to(dtype)
+    assert bool(torch.isfinite(x).all())
+    check(qm.gemm_w4(x.cuda(), packed.cuda(), scales.cuda(), group), x, q, scales, group)
